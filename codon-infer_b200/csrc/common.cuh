@@ -17,6 +17,7 @@ enum DeviceError : int {
   kDevBadArgs = 8,
   kDevTimeoutProbe = 16,
   kDevBadToken = 32,  // a token id outside [0, vocab): embedded as zeros, reported as an argument error
+  kDevBadSeqlens = 64,  // offsets of an operator's sequences that are not packed rows of its buffers: skipped
 };
 
 // Every spin-wait on an mbarrier gives up after this many nanoseconds of %globaltimer.

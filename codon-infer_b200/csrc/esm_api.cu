@@ -21,6 +21,7 @@
 #include "formats.h"
 #include "gemm_tc.cuh"
 #include "kernels.cuh"
+#include "train_ops.cuh"
 
 using esm::CodqHeader;
 
@@ -851,6 +852,8 @@ int check_device_word(esm_ctx* c) {
     cudaStreamSynchronize(c->stream);
     if (h == esm::kDevBadToken)
       return fail(c, ESM_EINVAL, "a token id is outside [0, " + std::to_string(c->cfg.vocab_size) + ")");
+    if (h == esm::kDevBadSeqlens)
+      return fail(c, ESM_EINVAL, "cu_seqlens are not ascending offsets of sequences of at most max_len rows");
     return fail(c, ESM_ETIMEOUT, "a device-side bounded wait gave up (code " + std::to_string(h) + ")");
   }
   return ESM_OK;
@@ -1778,6 +1781,397 @@ int esm_check_device(esm_ctx* c) {
   ESM_CUDA(cudaSetDevice(c->device));
   ESM_CUDA(cudaStreamSynchronize(c->stream));
   return check_device_word(c);
+}
+
+/* ---- operators on device memory ---------------------------------------------------------------- */
+
+namespace {
+
+// Makes the context's device current for one operator call and puts the caller's back.
+struct DeviceScope {
+  int before = -1;
+  cudaError_t rc = cudaSuccess;
+  explicit DeviceScope(int device) {
+    rc = cudaGetDevice(&before);
+    if (rc == cudaSuccess && before != device) rc = cudaSetDevice(device);
+    else if (rc == cudaSuccess) before = -1;
+  }
+  ~DeviceScope() {
+    if (before >= 0) cudaSetDevice(before);
+  }
+};
+
+size_t element_size(int type) { return type == ESM_F32 ? 4 : (type == ESM_F16 || type == ESM_BF16) ? 2 : 0; }
+
+// One buffer of an operator call: `rows` rows of `cols` elements of `size` bytes, `ld` elements apart.
+struct Buffer {
+  const char* name;
+  const void* p;
+  int64_t rows, cols, ld;
+  size_t size, align;
+  bool written;
+  bool optional = false;
+  uintptr_t begin() const { return reinterpret_cast<uintptr_t>(p); }
+  uintptr_t end() const {
+    return rows > 0 && cols > 0 ? begin() + (static_cast<uintptr_t>(rows - 1) * ld + cols) * size : begin();
+  }
+};
+
+// Every buffer given, aligned, on the context's device, rows not overlapping, and none that is
+// written shares memory with another one.
+int check_buffers(esm_ctx* c, const Buffer* b, int n, cudaStream_t s) {
+  if (s) {
+    // Asking a capturing stream for its device would end the capture; a launch on the stream of
+    // another device fails there by itself.
+    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+    int dev = c->device;
+    if (cudaStreamIsCapturing(s, &capture) != cudaSuccess ||
+        (capture == cudaStreamCaptureStatusNone && cudaStreamGetDevice(s, &dev) != cudaSuccess)) {
+      cudaGetLastError();
+      return fail(c, ESM_EINVAL, "not a stream");
+    }
+    if (dev != c->device) return fail(c, ESM_EINVAL, "the stream belongs to another device than the context");
+  }
+  for (int i = 0; i < n; ++i) {
+    const std::string name = b[i].name;
+    if (!b[i].p) {
+      if (b[i].optional) continue;
+      return fail(c, ESM_EINVAL, name + " is null");
+    }
+    if (b[i].ld < b[i].cols) return fail(c, ESM_EINVAL, name + ": the row stride is smaller than a row");
+    if (b[i].begin() % b[i].align || (b[i].align > b[i].size && b[i].rows > 1 && b[i].ld * b[i].size % b[i].align))
+      return fail(c, ESM_EINVAL, name + ": rows must start on " + std::to_string(b[i].align) + "-byte boundaries");
+    cudaPointerAttributes a{};
+    if (cudaPointerGetAttributes(&a, b[i].p) != cudaSuccess) {
+      cudaGetLastError();
+      return fail(c, ESM_EINVAL, name + " is not device memory");
+    }
+    if (a.type != cudaMemoryTypeManaged && (a.type != cudaMemoryTypeDevice || a.device != c->device))
+      return fail(c, ESM_EINVAL, name + " is not memory of the context's device");
+  }
+  for (int i = 0; i < n; ++i)
+    for (int j = i + 1; j < n; ++j)
+      if (b[i].p && b[j].p && (b[i].written || b[j].written) && b[i].begin() < b[j].end() && b[j].begin() < b[i].end())
+        return fail(c, ESM_EINVAL, std::string(b[i].name) + " and " + b[j].name + " overlap");
+  return ESM_OK;
+}
+
+int check_attention(esm_ctx* c, int32_t type, int32_t B, int32_t T, int32_t max_len, int32_t H, int32_t dh, float scale) {
+  if (type != ESM_F16 && type != ESM_BF16) return fail(c, ESM_EINVAL, "attention takes ESM_F16 or ESM_BF16");
+  if (B < 0 || T < 0 || max_len < 0 || max_len > T) return fail(c, ESM_EINVAL, "attention: bad B, T or max_len");
+  if (H <= 0 || H > 65535 || dh < 8 || dh > 64 || dh % 8)
+    return fail(c, ESM_EINVAL, "attention: head_dim must be a multiple of 8 up to 64 and n_heads positive");
+  if (!std::isfinite(scale)) return fail(c, ESM_EINVAL, "attention: scale must be finite");
+  if (B > 65535) return fail(c, ESM_EINVAL, "attention: more than 65535 sequences");
+  return ESM_OK;
+}
+
+int check_logits(esm_ctx* c, int32_t type, int32_t T, int32_t V, int32_t k, int32_t k_min) {
+  if (!element_size(type)) return fail(c, ESM_EINVAL, "unknown element type");
+  if (T < 0 || V <= 0) return fail(c, ESM_EINVAL, "bad number of rows or vocabulary size");
+  if (k < k_min || k > ESM_MAX_ALTERNATIVES || k > V)
+    return fail(c, ESM_EINVAL, "the number of alternatives must be in [" + std::to_string(k_min) + ", min(vocabulary, " +
+                                   std::to_string(ESM_MAX_ALTERNATIVES) + ")]");
+  return ESM_OK;
+}
+
+int check_layernorm(esm_ctx* c, int32_t x_type, int32_t y_type, int32_t T, int32_t d) {
+  if (!element_size(x_type) || !element_size(y_type)) return fail(c, ESM_EINVAL, "unknown element type");
+  if (T < 0 || d <= 0) return fail(c, ESM_EINVAL, "layernorm: bad number of rows or columns");
+  return ESM_OK;
+}
+
+}  // namespace
+
+int esm_attention(esm_ctx* c, int32_t type, const void* d_qkv, int64_t ld_qkv, const int32_t* d_cu_seqlens, int32_t B,
+                  int32_t T, int32_t max_len, int32_t n_heads, int32_t head_dim, float scale, void* d_out,
+                  int64_t ld_out, float* d_lse, void* stream) {
+  if (!c) return ESM_EINVAL;
+  std::lock_guard<std::mutex> lk(c->mu);
+  int rc = check_attention(c, type, B, T, max_len, n_heads, head_dim, scale);
+  if (rc) return rc;
+  if (B == 0 || T == 0 || max_len == 0) return ESM_OK;
+  const int64_t d = static_cast<int64_t>(n_heads) * head_dim;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  DeviceScope dev(c->device);
+  ESM_CUDA(dev.rc);
+  const Buffer bufs[] = {{"qkv", d_qkv, T, 3 * d, ld_qkv, 2, 16, false},
+                         {"cu_seqlens", d_cu_seqlens, 1, B + 1, B + 1, 4, 4, false},
+                         {"out", d_out, T, d, ld_out, 2, 16, true},
+                         {"lse", d_lse, n_heads, T, T, 4, 4, true, true}};
+  rc = check_buffers(c, bufs, 4, s);
+  if (rc) return rc;
+  esm::AttnOp p{};
+  p.dtype = type;
+  p.qkv = d_qkv;
+  p.ld_qkv = ld_qkv;
+  p.cu = d_cu_seqlens;
+  p.B = B;
+  p.T = T;
+  p.max_len = max_len;
+  p.H = n_heads;
+  p.dh = head_dim;
+  p.scale = scale;
+  p.out = d_out;
+  p.ld_out = ld_out;
+  p.lse = d_lse;
+  p.err = c->d_err;
+  ESM_CUDA(esm::launch_attention_op(p, s));
+  return ESM_OK;
+}
+
+int esm_attention_backward_workspace(int32_t B, int32_t T, int32_t n_heads, size_t* bytes) {
+  if (!bytes || B < 0 || T < 0 || n_heads <= 0) return ESM_EINVAL;
+  *bytes = esm::attention_backward_bytes(B, T, n_heads);
+  return ESM_OK;
+}
+
+int esm_attention_backward(esm_ctx* c, int32_t type, const void* d_qkv, int64_t ld_qkv, const int32_t* d_cu_seqlens,
+                           int32_t B, int32_t T, int32_t max_len, int32_t n_heads, int32_t head_dim, float scale,
+                           const void* d_out, int64_t ld_out, const float* d_lse, const void* d_dout, int64_t ld_dout,
+                           void* d_dqkv, int64_t ld_dqkv, void* d_workspace, size_t workspace_bytes, void* stream) {
+  if (!c) return ESM_EINVAL;
+  std::lock_guard<std::mutex> lk(c->mu);
+  int rc = check_attention(c, type, B, T, max_len, n_heads, head_dim, scale);
+  if (rc) return rc;
+  if (B == 0 || T == 0 || max_len == 0) return ESM_OK;
+  const size_t need = esm::attention_backward_bytes(B, T, n_heads);
+  if (workspace_bytes < need)
+    return fail(c, ESM_ECAPACITY, "attention backward needs a workspace of " + std::to_string(need) + " bytes");
+  const int64_t d = static_cast<int64_t>(n_heads) * head_dim;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  DeviceScope dev(c->device);
+  ESM_CUDA(dev.rc);
+  const Buffer bufs[] = {{"qkv", d_qkv, T, 3 * d, ld_qkv, 2, 16, false},
+                         {"cu_seqlens", d_cu_seqlens, 1, B + 1, B + 1, 4, 4, false},
+                         {"out", d_out, T, d, ld_out, 2, 16, false},
+                         {"lse", d_lse, n_heads, T, T, 4, 4, false},
+                         {"dout", d_dout, T, d, ld_dout, 2, 16, false},
+                         {"dqkv", d_dqkv, T, 3 * d, ld_dqkv, 2, 16, true},
+                         {"workspace", d_workspace, 1, static_cast<int64_t>(need), static_cast<int64_t>(need), 1, 16, true}};
+  rc = check_buffers(c, bufs, 7, s);
+  if (rc) return rc;
+  esm::AttnOp p{};
+  p.dtype = type;
+  p.qkv = d_qkv;
+  p.ld_qkv = ld_qkv;
+  p.cu = d_cu_seqlens;
+  p.B = B;
+  p.T = T;
+  p.max_len = max_len;
+  p.H = n_heads;
+  p.dh = head_dim;
+  p.scale = scale;
+  p.out = const_cast<void*>(d_out);
+  p.ld_out = ld_out;
+  p.lse = const_cast<float*>(d_lse);
+  p.dout = d_dout;
+  p.ld_dout = ld_dout;
+  p.dqkv = d_dqkv;
+  p.ld_dqkv = ld_dqkv;
+  p.workspace = static_cast<float*>(d_workspace);
+  p.err = c->d_err;
+  ESM_CUDA(esm::launch_attention_backward(p, s));
+  return ESM_OK;
+}
+
+int esm_layernorm(esm_ctx* c, int32_t x_type, int32_t y_type, const void* d_x, const float* d_w, const float* d_b,
+                  float eps, int32_t T, int32_t d, void* d_y, float* d_mean, float* d_rstd, void* stream) {
+  if (!c) return ESM_EINVAL;
+  std::lock_guard<std::mutex> lk(c->mu);
+  int rc = check_layernorm(c, x_type, y_type, T, d);
+  if (rc) return rc;
+  if (!(eps >= 0.0f) || !std::isfinite(eps)) return fail(c, ESM_EINVAL, "layernorm: eps must be finite and not negative");
+  if (T == 0) return ESM_OK;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  DeviceScope dev(c->device);
+  ESM_CUDA(dev.rc);
+  const size_t ex = element_size(x_type), ey = element_size(y_type);
+  const Buffer bufs[] = {{"x", d_x, T, d, d, ex, ex, false},         {"w", d_w, 1, d, d, 4, 4, false},
+                         {"b", d_b, 1, d, d, 4, 4, false},           {"y", d_y, T, d, d, ey, ey, true},
+                         {"mean", d_mean, 1, T, T, 4, 4, true, true}, {"rstd", d_rstd, 1, T, T, 4, 4, true, true}};
+  rc = check_buffers(c, bufs, 6, s);
+  if (rc) return rc;
+  esm::LayerNormOp p{};
+  p.x_type = x_type;
+  p.y_type = y_type;
+  p.x = d_x;
+  p.w = d_w;
+  p.b = d_b;
+  p.eps = eps;
+  p.T = T;
+  p.d = d;
+  p.y = d_y;
+  p.mean = d_mean;
+  p.rstd = d_rstd;
+  p.num_sms = c->num_sms;
+  ESM_CUDA(esm::launch_layernorm_op(p, s));
+  return ESM_OK;
+}
+
+int esm_layernorm_backward_workspace(const esm_ctx* c, int32_t T, int32_t d, size_t* bytes) {
+  if (!c || !bytes || T < 0 || d <= 0) return ESM_EINVAL;
+  *bytes = esm::layernorm_backward_bytes(T, d, c->num_sms);
+  return ESM_OK;
+}
+
+int esm_layernorm_backward(esm_ctx* c, int32_t x_type, int32_t y_type, const void* d_dy, const void* d_x,
+                           const float* d_w, const float* d_mean, const float* d_rstd, const void* d_dres, int32_t T,
+                           int32_t d, void* d_dx, float* d_dw, float* d_db, void* d_workspace, size_t workspace_bytes,
+                           void* stream) {
+  if (!c) return ESM_EINVAL;
+  std::lock_guard<std::mutex> lk(c->mu);
+  int rc = check_layernorm(c, x_type, y_type, T, d);
+  if (rc) return rc;
+  const size_t need = esm::layernorm_backward_bytes(T, d, c->num_sms);
+  if (workspace_bytes < need)
+    return fail(c, ESM_ECAPACITY, "layernorm backward needs a workspace of " + std::to_string(need) + " bytes");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  DeviceScope dev(c->device);
+  ESM_CUDA(dev.rc);
+  const size_t ex = element_size(x_type), ey = element_size(y_type);
+  const bool none = T == 0;  // no rows: the weights' gradients are zero
+  const Buffer bufs[] = {
+      {"dy", d_dy, T, d, d, ey, ey, false, none},    {"x", d_x, T, d, d, ex, ex, false, none},
+      {"w", d_w, 1, d, d, 4, 4, false},              {"mean", d_mean, 1, T, T, 4, 4, false, none},
+      {"rstd", d_rstd, 1, T, T, 4, 4, false, none},  {"dres", d_dres, T, d, d, ex, ex, false, true},
+      {"dx", d_dx, T, d, d, ex, ex, true, none},     {"dw", d_dw, 1, d, d, 4, 4, true},
+      {"db", d_db, 1, d, d, 4, 4, true},
+      {"workspace", d_workspace, 1, static_cast<int64_t>(need), static_cast<int64_t>(need), 1, 16, true}};
+  rc = check_buffers(c, bufs, 10, s);
+  if (rc) return rc;
+  esm::LayerNormOp p{};
+  p.x_type = x_type;
+  p.y_type = y_type;
+  p.x = d_x;
+  p.w = d_w;
+  p.T = T;
+  p.d = d;
+  p.mean = const_cast<float*>(d_mean);
+  p.rstd = const_cast<float*>(d_rstd);
+  p.dy = d_dy;
+  p.dres = d_dres;
+  p.dx = d_dx;
+  p.dw = d_dw;
+  p.db = d_db;
+  p.workspace = static_cast<float*>(d_workspace);
+  p.num_sms = c->num_sms;
+  ESM_CUDA(esm::launch_layernorm_backward(p, s));
+  return ESM_OK;
+}
+
+int esm_token_logprobs(esm_ctx* c, int32_t type, const void* d_logits, int64_t ld, int32_t T, int32_t V,
+                       const int32_t* d_targets, int32_t k, float* d_logp, float* d_entropy, int32_t* d_top_ids,
+                       float* d_top_logp, void* stream) {
+  if (!c) return ESM_EINVAL;
+  std::lock_guard<std::mutex> lk(c->mu);
+  int rc = check_logits(c, type, T, V, k, 0);
+  if (rc) return rc;
+  if (!d_targets != !d_logp) return fail(c, ESM_EINVAL, "targets and logp go together");
+  if (T == 0) return ESM_OK;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  DeviceScope dev(c->device);
+  ESM_CUDA(dev.rc);
+  const size_t e = element_size(type);
+  const Buffer bufs[] = {{"logits", d_logits, T, V, ld, e, e, false},
+                         {"targets", d_targets, 1, T, T, 4, 4, false, true},
+                         {"logp", d_logp, 1, T, T, 4, 4, true, true},
+                         {"entropy", d_entropy, 1, T, T, 4, 4, true, true},
+                         {"top_ids", d_top_ids, T, k, k, 4, 4, true, k == 0},
+                         {"top_logp", d_top_logp, T, k, k, 4, 4, true, k == 0}};
+  rc = check_buffers(c, bufs, 6, s);
+  if (rc) return rc;
+  esm::LogitsOp p{};
+  p.dtype = type;
+  p.logits = d_logits;
+  p.ld = ld;
+  p.T = T;
+  p.V = V;
+  p.k = k;
+  p.targets = d_targets;
+  p.logp = d_logp;
+  p.entropy = d_entropy;
+  p.top_ids = d_top_ids;
+  p.top_logp = d_top_logp;
+  ESM_CUDA(esm::launch_token_logprobs(p, s));
+  return ESM_OK;
+}
+
+int esm_distill_loss(esm_ctx* c, int32_t type, const void* d_logits, int64_t ld, int32_t T, int32_t V,
+                     const int32_t* d_top_ids, const float* d_top_logits, int32_t k, float temperature, float* d_loss,
+                     float* d_lse, void* stream) {
+  if (!c) return ESM_EINVAL;
+  std::lock_guard<std::mutex> lk(c->mu);
+  int rc = check_logits(c, type, T, V, k, 1);
+  if (rc) return rc;
+  if (!(temperature > 0.0f) || !std::isfinite(temperature))
+    return fail(c, ESM_EINVAL, "distillation: the temperature must be positive and finite");
+  if (T == 0) return ESM_OK;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  DeviceScope dev(c->device);
+  ESM_CUDA(dev.rc);
+  const size_t e = element_size(type);
+  const Buffer bufs[] = {{"logits", d_logits, T, V, ld, e, e, false},
+                         {"top_ids", d_top_ids, T, k, k, 4, 4, false},
+                         {"top_logits", d_top_logits, T, k, k, 4, 4, false},
+                         {"loss", d_loss, 1, T, T, 4, 4, true},
+                         {"lse", d_lse, 1, T, T, 4, 4, true}};
+  rc = check_buffers(c, bufs, 5, s);
+  if (rc) return rc;
+  esm::LogitsOp p{};
+  p.dtype = type;
+  p.logits = d_logits;
+  p.ld = ld;
+  p.T = T;
+  p.V = V;
+  p.k = k;
+  p.alt_ids = d_top_ids;
+  p.alt_logits = d_top_logits;
+  p.temperature = temperature;
+  p.loss = d_loss;
+  p.lse = d_lse;
+  ESM_CUDA(esm::launch_distill_loss(p, s));
+  return ESM_OK;
+}
+
+int esm_distill_backward(esm_ctx* c, int32_t type, const void* d_logits, int64_t ld, int32_t T, int32_t V,
+                         const int32_t* d_top_ids, const float* d_top_logits, int32_t k, float temperature,
+                         const float* d_lse, const float* d_dloss, void* d_dlogits, int64_t ld_grad, void* stream) {
+  if (!c) return ESM_EINVAL;
+  std::lock_guard<std::mutex> lk(c->mu);
+  int rc = check_logits(c, type, T, V, k, 1);
+  if (rc) return rc;
+  if (!(temperature > 0.0f) || !std::isfinite(temperature))
+    return fail(c, ESM_EINVAL, "distillation: the temperature must be positive and finite");
+  if (T == 0) return ESM_OK;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  DeviceScope dev(c->device);
+  ESM_CUDA(dev.rc);
+  const size_t e = element_size(type);
+  const Buffer bufs[] = {{"logits", d_logits, T, V, ld, e, e, false},
+                         {"top_ids", d_top_ids, T, k, k, 4, 4, false},
+                         {"top_logits", d_top_logits, T, k, k, 4, 4, false},
+                         {"lse", d_lse, 1, T, T, 4, 4, false},
+                         {"dloss", d_dloss, 1, T, T, 4, 4, false},
+                         {"dlogits", d_dlogits, T, V, ld_grad, e, e, true}};
+  rc = check_buffers(c, bufs, 6, s);
+  if (rc) return rc;
+  esm::LogitsOp p{};
+  p.dtype = type;
+  p.logits = d_logits;
+  p.ld = ld;
+  p.T = T;
+  p.V = V;
+  p.k = k;
+  p.alt_ids = d_top_ids;
+  p.alt_logits = d_top_logits;
+  p.temperature = temperature;
+  p.lse = const_cast<float*>(d_lse);
+  p.dloss = d_dloss;
+  p.dlogits = d_dlogits;
+  p.ld_grad = ld_grad;
+  ESM_CUDA(esm::launch_distill_backward(p, s));
+  return ESM_OK;
 }
 
 }  // extern "C"

@@ -24,6 +24,8 @@ DTYPE_FP32, DTYPE_Q8_0, DTYPE_Q4_0, DTYPE_Q3_LUT = 0, 1, 2, 3
 ARCH_8M, ARCH_35M, ARCH_150M, ARCH_650M, ARCH_3B = range(5)
 Q8_BLOCK_BYTES, Q4_BLOCK_BYTES = 36, 20
 MASK_ID = 32
+TYPE_F32, TYPE_F16, TYPE_BF16 = 0, 1, 2  # element types of the operators' matrices (ESM_F32 ..)
+MAX_ALTERNATIVES = 64
 
 # EsmWeights field order (also the grouped_canonical_v1 / CODQ file order).
 TENSOR_NAMES = (
@@ -96,6 +98,7 @@ def lib() -> ctypes.CDLL:
                                "(there is no CPU fallback)")
         L = ctypes.CDLL(str(LIB_PATH))
         vp, i32, i64, f32 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_float
+        sz = ctypes.c_size_t
         sig = {
             "esm_config_preset": [i32, vp],
             "esm_config_detect_file": [ctypes.c_char_p, vp, vp],
@@ -133,6 +136,16 @@ def lib() -> ctypes.CDLL:
             "esm_group_reserve": [vp, i32, i32, i32, i32],
             "esm_group_forward": [vp, vp, vp, i32, i32, vp, vp, vp],
             "esm_group_dms_masked_marginal": [vp, vp, i32, i32, vp, vp],
+            "esm_attention": [vp, i32, vp, i64, vp, i32, i32, i32, i32, i32, f32, vp, i64, vp, vp],
+            "esm_attention_backward_workspace": [i32, i32, i32, vp],
+            "esm_attention_backward": [vp, i32, vp, i64, vp, i32, i32, i32, i32, i32, f32, vp, i64, vp, vp, i64, vp, i64,
+                                       vp, sz, vp],
+            "esm_layernorm": [vp, i32, i32, vp, vp, vp, f32, i32, i32, vp, vp, vp, vp],
+            "esm_layernorm_backward_workspace": [vp, i32, i32, vp],
+            "esm_layernorm_backward": [vp, i32, i32, vp, vp, vp, vp, vp, vp, i32, i32, vp, vp, vp, vp, sz, vp],
+            "esm_token_logprobs": [vp, i32, vp, i64, i32, i32, vp, i32, vp, vp, vp, vp, vp],
+            "esm_distill_loss": [vp, i32, vp, i64, i32, i32, vp, vp, i32, f32, vp, vp, vp],
+            "esm_distill_backward": [vp, i32, vp, i64, i32, i32, vp, vp, i32, f32, vp, vp, vp, i64, vp],
             "esm_check_device": [vp],
             "esm_probe_wait_timeout": [vp, i32],
             "esm_profile_enable": [vp, i32],
@@ -158,6 +171,56 @@ def _check(rc: int, what: str, ctx=None) -> None:
 
 def _p(a):
     return None if a is None else ctypes.c_void_p(a.ctypes.data)
+
+
+# ---- tensors of the operators on device memory ------------------------------------------------
+
+_ELEMENT_TYPES = {"float32": TYPE_F32, "float16": TYPE_F16, "bfloat16": TYPE_BF16, "int32": -1}
+_type_of: dict = {}  # dtype object -> element type
+
+
+def _element_type(t) -> int:
+    ty = _type_of.get(t.dtype)
+    if ty is None:
+        name = str(t.dtype).rsplit(".", 1)[-1]
+        if name not in _ELEMENT_TYPES:
+            raise EsmError(ESM_EINVAL, f"element type {t.dtype} is not supported")
+        ty = _type_of[t.dtype] = _ELEMENT_TYPES[name]
+    return ty
+
+
+def _bad(what: str):
+    raise EsmError(ESM_EINVAL, what)
+
+
+def _rows(t, name: str, shape: tuple, types=None) -> tuple[int, int, int]:
+    """(pointer, row stride, element type) of a CUDA matrix of `shape` whose rows are contiguous."""
+    if tuple(t.shape) != shape:
+        _bad(f"{name} must have the shape {shape}, not {tuple(t.shape)}")
+    ty = _element_type(t)
+    if types is not None and ty not in types:
+        _bad(f"{name} has the element type {t.dtype}")
+    ld, inner = t.stride()
+    if shape[1] > 1 and inner != 1:
+        _bad(f"{name}: rows must be contiguous")
+    return t.data_ptr(), (ld if shape[0] > 1 else shape[1]), ty
+
+
+def _flat(t, name: str, shape: tuple, ty: int = TYPE_F32):
+    """Pointer of a contiguous CUDA tensor of `shape` and element type `ty` (None stays None)."""
+    if t is None:
+        return None
+    if tuple(t.shape) != shape:
+        _bad(f"{name} must have the shape {shape}, not {tuple(t.shape)}")
+    if _element_type(t) != ty:
+        _bad(f"{name} has the element type {t.dtype}")
+    if not t.is_contiguous():
+        _bad(f"{name} must be contiguous")
+    return t.data_ptr()
+
+
+def _stream(stream):
+    return None if stream is None else (stream if isinstance(stream, int) else stream.cuda_stream)
 
 
 # ---- quantizers / tokenizer ------------------------------------------------------------------
@@ -462,6 +525,119 @@ class Model:
         self._chk(lib().esm_matmul_tiled(self._ctx, dtype, _p(x), _p(w), _p(b), in_dim, out_dim, seq_len, _p(out)),
                   "esm_matmul_tiled")
         return out
+
+    # Operators on CUDA tensors (torch tensors, or any with data_ptr, shape, stride and dtype). Outputs
+    # are the caller's tensors; calls are enqueued on `stream` (None: the legacy default stream) and
+    # do not wait. See include/esm_b200.h for the formulas and limits.
+
+    def attention(self, qkv, cu_seqlens, max_len: int, n_heads: int, out, lse=None, scale: float | None = None,
+                  stream=None) -> None:
+        """Attention of packed sequences: qkv [T, 3 d] -> out [T, d], lse [n_heads, T] (or None);
+        cu_seqlens int32 [B + 1] on the device; scale defaults to head_dim^-1/2."""
+        T, d = out.shape
+        dh = self._head_dim(d, n_heads)
+        q, ldq, ty = _rows(qkv, "qkv", (T, 3 * d))
+        o, ldo, _ = _rows(out, "out", (T, d), (ty,))
+        B = cu_seqlens.shape[0] - 1
+        rc = lib().esm_attention(self._ctx, ty, q, ldq, _flat(cu_seqlens, "cu_seqlens", (B + 1,), -1), B, T, max_len,
+                                 n_heads, dh, dh ** -0.5 if scale is None else scale, o, ldo,
+                                 _flat(lse, "lse", (n_heads, T)), _stream(stream))
+        self._chk(rc, "esm_attention")
+
+    @staticmethod
+    def _head_dim(d: int, n_heads: int) -> int:
+        if n_heads <= 0 or d % n_heads:
+            _bad(f"{d} columns do not divide into {n_heads} heads")
+        return d // n_heads
+
+    @staticmethod
+    def attention_backward_workspace(batch: int, rows: int, n_heads: int) -> int:
+        n = ctypes.c_size_t()
+        _check(lib().esm_attention_backward_workspace(batch, rows, n_heads, ctypes.byref(n)),
+               "esm_attention_backward_workspace")
+        return n.value
+
+    def attention_backward(self, qkv, cu_seqlens, max_len: int, n_heads: int, out, lse, dout, dqkv, workspace,
+                           scale: float | None = None, stream=None) -> None:
+        """Gradient dqkv [T, 3 d] of attention's qkv from dout [T, d]; out and lse as attention wrote
+        them; workspace: a contiguous tensor of attention_backward_workspace(B, T, n_heads) bytes."""
+        T, d = out.shape
+        dh = self._head_dim(d, n_heads)
+        q, ldq, ty = _rows(qkv, "qkv", (T, 3 * d))
+        o, ldo, _ = _rows(out, "out", (T, d), (ty,))
+        g, ldg, _ = _rows(dout, "dout", (T, d), (ty,))
+        dq, lddq, _ = _rows(dqkv, "dqkv", (T, 3 * d), (ty,))
+        B = cu_seqlens.shape[0] - 1
+        rc = lib().esm_attention_backward(self._ctx, ty, q, ldq, _flat(cu_seqlens, "cu_seqlens", (B + 1,), -1), B, T,
+                                          max_len, n_heads, dh, dh ** -0.5 if scale is None else scale, o, ldo,
+                                          _flat(lse, "lse", (n_heads, T)), g, ldg, dq, lddq, workspace.data_ptr(),
+                                          workspace.numel() * workspace.element_size(), _stream(stream))
+        self._chk(rc, "esm_attention_backward")
+
+    def layernorm(self, x, w, b, y, mean=None, rstd=None, eps: float = 1e-5, stream=None) -> None:
+        """y [T, d] = LayerNorm of the rows of x [T, d]; w, b [d], mean and rstd [T] in float32."""
+        T, d = x.shape
+        rc = lib().esm_layernorm(self._ctx, _element_type(x), _element_type(y), _flat(x, "x", (T, d), _element_type(x)),
+                                 _flat(w, "w", (d,)), _flat(b, "b", (d,)), eps, T, d,
+                                 _flat(y, "y", (T, d), _element_type(y)), _flat(mean, "mean", (T,)),
+                                 _flat(rstd, "rstd", (T,)), _stream(stream))
+        self._chk(rc, "esm_layernorm")
+
+    def layernorm_backward_workspace(self, rows: int, dim: int) -> int:
+        n = ctypes.c_size_t()
+        self._chk(lib().esm_layernorm_backward_workspace(self._ctx, rows, dim, ctypes.byref(n)),
+                  "esm_layernorm_backward_workspace")
+        return n.value
+
+    def layernorm_backward(self, dy, x, w, mean, rstd, dx, dw, db, workspace, dres=None, stream=None) -> None:
+        """Gradients dx [T, d] (plus dres, the gradient past the LayerNorm, when given), dw and db [d]
+        from dy [T, d]; workspace: a contiguous tensor of layernorm_backward_workspace(T, d) bytes."""
+        T, d = x.shape
+        xt, yt = _element_type(x), _element_type(dy)
+        rc = lib().esm_layernorm_backward(self._ctx, xt, yt, _flat(dy, "dy", (T, d), yt), _flat(x, "x", (T, d), xt),
+                                          _flat(w, "w", (d,)), _flat(mean, "mean", (T,)), _flat(rstd, "rstd", (T,)),
+                                          _flat(dres, "dres", (T, d), xt), T, d, _flat(dx, "dx", (T, d), xt),
+                                          _flat(dw, "dw", (d,)), _flat(db, "db", (d,)), workspace.data_ptr(),
+                                          workspace.numel() * workspace.element_size(), _stream(stream))
+        self._chk(rc, "esm_layernorm_backward")
+
+    def token_logprobs(self, logits, targets=None, logp=None, entropy=None, top_ids=None, top_logp=None,
+                       stream=None) -> None:
+        """Log probabilities of the rows of logits [T, V]: logp [T] of targets [T] (int32), entropy [T],
+        and the most probable tokens top_ids [T, k] (int32) with top_logp [T, k]; each may be None."""
+        T, V = logits.shape
+        x, ld, ty = _rows(logits, "logits", (T, V))
+        k = 0 if top_ids is None else top_ids.shape[1]
+        if (top_ids is None) != (top_logp is None):
+            _bad("top_ids and top_logp go together")
+        rc = lib().esm_token_logprobs(self._ctx, ty, x, ld, T, V, _flat(targets, "targets", (T,), -1), k,
+                                      _flat(logp, "logp", (T,)), _flat(entropy, "entropy", (T,)),
+                                      _flat(top_ids, "top_ids", (T, k), -1), _flat(top_logp, "top_logp", (T, k)),
+                                      _stream(stream))
+        self._chk(rc, "esm_token_logprobs")
+
+    def distill_loss(self, logits, top_ids, top_logits, loss, lse, temperature: float = 1.0, stream=None) -> None:
+        """loss [T] of the student's logits [T, V] against a teacher's alternatives top_ids (int32) and
+        top_logits [T, k], and lse [T] for distill_backward."""
+        T, V = logits.shape
+        x, ld, ty = _rows(logits, "logits", (T, V))
+        k = top_ids.shape[1]
+        rc = lib().esm_distill_loss(self._ctx, ty, x, ld, T, V, _flat(top_ids, "top_ids", (T, k), -1),
+                                    _flat(top_logits, "top_logits", (T, k)), k, temperature, _flat(loss, "loss", (T,)),
+                                    _flat(lse, "lse", (T,)), _stream(stream))
+        self._chk(rc, "esm_distill_loss")
+
+    def distill_backward(self, logits, top_ids, top_logits, lse, dloss, dlogits, temperature: float = 1.0,
+                         stream=None) -> None:
+        """dlogits [T, V], the gradient of sum_t dloss[t] * loss[t]; lse as distill_loss wrote it."""
+        T, V = logits.shape
+        x, ld, ty = _rows(logits, "logits", (T, V))
+        dx, ldg, _ = _rows(dlogits, "dlogits", (T, V), (ty,))
+        k = top_ids.shape[1]
+        rc = lib().esm_distill_backward(self._ctx, ty, x, ld, T, V, _flat(top_ids, "top_ids", (T, k), -1),
+                                        _flat(top_logits, "top_logits", (T, k)), k, temperature,
+                                        _flat(lse, "lse", (T,)), _flat(dloss, "dloss", (T,)), dx, ldg, _stream(stream))
+        self._chk(rc, "esm_distill_backward")
 
     def profile_enable(self, on: bool = True) -> None:
         self._chk(lib().esm_profile_enable(self._ctx, int(on)), "esm_profile_enable")

@@ -247,6 +247,108 @@ int esm_matmul_tiled(esm_ctx* ctx, int32_t dtype, const float* x, const void* w,
 int esm_matmul_tiled_noalloc(int32_t dtype, const float* d_x, const void* d_w, const float* d_bias, int32_t in_dim,
                              int32_t out_dim, int32_t seq_len, float* d_out, void* stream);
 
+/* ---- training and scoring operators on device memory (no counterpart in the reference) --------- */
+
+/* What a distillation or fine-tuning step of the encoder needs around its GEMMs: attention over
+ * packed sequences with its backward pass, LayerNorm with its backward pass, per-token log
+ * probabilities, and the loss of a student against a teacher's top alternatives with its gradient.
+ *
+ * All of them: buffers are DEVICE memory of the context's GPU, rows are row-major, `ld` arguments
+ * are row strides in elements. A call is enqueued on `stream` (a cudaStream_t of that GPU; NULL =
+ * the legacy default stream), allocates nothing and does not wait, so it may be captured into a CUDA
+ * graph; it does not change the calling thread's current device. A null, misaligned, foreign-device
+ * or host pointer, or a buffer that is written and overlaps another one, is ESM_EINVAL; a workspace
+ * that is too small is ESM_ECAPACITY. A workspace holds nothing between calls; calls that may run
+ * at the same time (two streams, two captured graphs) need one each. Results do not depend on how
+ * often or beside what a call runs: sums are taken in a fixed order. Calls with no rows do nothing
+ * (esm_layernorm_backward then writes zero weight gradients). */
+
+/* Element types of the operators' matrices (not the ESM_DTYPE_* storage types of weights). */
+enum { ESM_F32 = 0, ESM_F16 = 1, ESM_BF16 = 2 };
+
+/* Attention of every sequence over its own rows, as in the encoder's layers (bidirectional; the
+ * key-padding mask is implied by the packing): per head h of H = n_heads,
+ *   S = scale Q K^T,  lse_i = log sum_j exp(S_ij),  out = exp(S - lse) V.
+ * d_qkv [T, 3 H head_dim] of `type` (ESM_F16 or ESM_BF16): queries, keys and values, head h at columns
+ * h * head_dim of each part; d_out [T, H head_dim]; both with rows on 16-byte boundaries. d_cu_seqlens
+ * [B + 1] (int32, DEVICE memory): sequence b is rows cu[b] .. cu[b + 1], empty ones allowed; max_len
+ * bounds their lengths. T is the number of rows of the buffers: rows behind the last sequence are
+ * left as they are. head_dim is a multiple of 8 up to 64; B and n_heads at most 65535. d_lse [H, T] or NULL (the
+ * backward pass needs it). Scores, sums and outputs are accumulated in fp32, probabilities are rounded to
+ * `type` for the product with V. Offsets that do not fit (descending, beyond T or longer than
+ * max_len) are noticed on the device: that sequence is skipped and esm_check_device returns
+ * ESM_EINVAL. */
+int esm_attention(esm_ctx* ctx, int32_t type, const void* d_qkv, int64_t ld_qkv, const int32_t* d_cu_seqlens,
+                  int32_t B, int32_t T, int32_t max_len, int32_t n_heads, int32_t head_dim, float scale, void* d_out,
+                  int64_t ld_out, float* d_lse, void* stream);
+
+/* Its backward pass: from d_dout [T, H head_dim], the gradient of out, d_dqkv [T, 3 H head_dim], the
+ * gradients of queries, keys and values in the layout of d_qkv. d_out and d_lse are those of
+ * esm_attention on the same d_qkv; the probabilities are computed again from them:
+ *   P = exp(S - lse),  D = rowsum(dout out),  dV = P^T dout,
+ *   dS = P (dout V^T - D),  dQ = scale dS K,  dK = scale dS^T Q.
+ * P and dS are rounded to `type` for the products; with ESM_F16 each is scaled by a power of two
+ * first (from the largest |dout| and |V| of the sequence and head), so small gradients do not
+ * underflow. d_workspace: esm_attention_backward_workspace bytes, 16-byte aligned. */
+int esm_attention_backward_workspace(int32_t B, int32_t T, int32_t n_heads, size_t* bytes);
+int esm_attention_backward(esm_ctx* ctx, int32_t type, const void* d_qkv, int64_t ld_qkv,
+                           const int32_t* d_cu_seqlens, int32_t B, int32_t T, int32_t max_len, int32_t n_heads,
+                           int32_t head_dim, float scale, const void* d_out, int64_t ld_out, const float* d_lse,
+                           const void* d_dout, int64_t ld_dout, void* d_dqkv, int64_t ld_dqkv, void* d_workspace,
+                           size_t workspace_bytes, void* stream);
+
+/* LayerNorm of T rows of d elements (contiguous), as the encoder's: mean = sum x / d, rstd = (sum
+ * (x - mean)^2 / d + eps)^-1/2, y = (x - mean) rstd w + b. x and y have their own element types; w,
+ * b [d] and the statistics [T] are fp32. d_mean and d_rstd may be NULL (the backward pass needs
+ * them). */
+int esm_layernorm(esm_ctx* ctx, int32_t x_type, int32_t y_type, const void* d_x, const float* d_w, const float* d_b,
+                  float eps, int32_t T, int32_t d, void* d_y, float* d_mean, float* d_rstd, void* stream);
+
+/* Its backward pass: from d_dy [T, d] of y_type, with g = dy w and xh = (x - mean) rstd,
+ *   dx = rstd (g - mean(g) - xh mean(g xh)) + dres,  dw = sum over rows of dy xh,  db = sum over rows of dy.
+ * d_dx [T, d] and d_dres have x_type; d_dres (the gradient that reaches x past the LayerNorm, as in a
+ * pre-LayerNorm residual block) may be NULL. d_dw and d_db [d] are fp32. d_workspace:
+ * esm_layernorm_backward_workspace bytes, 16-byte aligned. */
+int esm_layernorm_backward_workspace(const esm_ctx* ctx, int32_t T, int32_t d, size_t* bytes);
+int esm_layernorm_backward(esm_ctx* ctx, int32_t x_type, int32_t y_type, const void* d_dy, const void* d_x,
+                           const float* d_w, const float* d_mean, const float* d_rstd, const void* d_dres, int32_t T,
+                           int32_t d, void* d_dx, float* d_dw, float* d_db, void* d_workspace, size_t workspace_bytes,
+                           void* stream);
+
+/* The most alternatives (top tokens) of a row. */
+#define ESM_MAX_ALTERNATIVES 64
+
+/* Log probabilities of T rows of V logits of `type` (e.g. esm_forward_device's d_logits, ESM_F32), over
+ * the whole vocabulary: d_logp[t] that of token d_targets[t] (0 where the target is outside [0, V):
+ * padding), both NULL or neither; d_entropy[t] the distribution's entropy in nats, or NULL; and the
+ * k <= min(V, ESM_MAX_ALTERNATIVES) most probable tokens of each row, d_top_ids and d_top_logp
+ * [T, k], in descending order with ties in id order (k = 0: none). Logits of -inf are tokens that
+ * cannot occur. A row without a distribution (a NaN or +inf among its logits, or none above -inf) has
+ * NaN log probabilities and entropy, and top ids of -1. */
+int esm_token_logprobs(esm_ctx* ctx, int32_t type, const void* d_logits, int64_t ld, int32_t T, int32_t V,
+                       const int32_t* d_targets, int32_t k, float* d_logp, float* d_entropy, int32_t* d_top_ids,
+                       float* d_top_logp, void* stream);
+
+/* Distillation loss of T rows of student logits [T, V] against a teacher's alternatives, k per row
+ * (esm_token_logprobs' d_top_ids and d_top_logp of the teacher, or its logits at those ids): with
+ * q = softmax(logits / temperature) over the vocabulary and p = softmax(top_logits / temperature) over
+ * the row's alternatives,
+ *   loss[t] = temperature^2 sum_i p_i (log p_i - log q[id_i]).
+ * An alternative whose id is outside [0, V) is absent, and its d_top_logits entry is ignored; a row
+ * without any (or with none above -inf) has loss 0. An id that is given twice counts with both its
+ * probabilities. d_lse[t] = log sum_j exp(logits[t, j] / temperature), for the gradient. */
+int esm_distill_loss(esm_ctx* ctx, int32_t type, const void* d_logits, int64_t ld, int32_t T, int32_t V,
+                     const int32_t* d_top_ids, const float* d_top_logits, int32_t k, float temperature, float* d_loss,
+                     float* d_lse, void* stream);
+
+/* Its gradient: d_dlogits [T, V] (row stride ld_grad) of `type`,
+ *   dlogits[t, j] = dloss[t] temperature (q_j - sum of the p_i with id_i = j),
+ * from the same arguments, d_lse of esm_distill_loss and the gradient d_dloss [T] of each row's loss.
+ * A row whose dloss is 0 (padding), or that has no alternatives, gets zeros whatever its logits are. */
+int esm_distill_backward(esm_ctx* ctx, int32_t type, const void* d_logits, int64_t ld, int32_t T, int32_t V,
+                         const int32_t* d_top_ids, const float* d_top_logits, int32_t k, float temperature,
+                         const float* d_lse, const float* d_dloss, void* d_dlogits, int64_t ld_grad, void* stream);
+
 /* ---- several GPUs from one host process ------------------------------------------------------ */
 
 /* The reference runs every sequence and every masked variant of a scan as its own forward, one
