@@ -27,9 +27,13 @@
 // step's row sum against it exceeds p.rescale_sum; EXP 0..2: a step's row max exceeds it by more
 // than 2^8), after PV(j - 1) has completed. All waits are bounded.
 #include <atomic>
+#include <type_traits>
 
 #include "common.cuh"
+#include "gemm_tc.cuh"
 #include "kernels.cuh"
+#include "train_common.cuh"
+#include "train_ops.cuh"
 
 namespace esm {
 
@@ -77,15 +81,21 @@ __device__ __forceinline__ uint32_t o_col(int t) { return static_cast<uint32_t>(
 // which leaves only the products of two residues out of the fp32 score. (With peaked attention,
 // as in trained models, fp16 queries and keys alone move the scores of the dominant keys by a few
 // hundredths and the logits by about 1e-2.) Other head sizes pass tmap_q / tmap_kv again there.
-template <int DH, int POLY, int EXP, bool PAD, int SPLIT>
+// OP: the attention operator on a caller's buffers (launch_attention_op). Its heads, of any width up
+// to DH and elements E, always arrive through 3-D maps, with plain scores; blocks are (256-query block, head,
+// sequence) of device-side offsets that are checked here; and neither the rows nor the numbers of
+// other sequences may reach a result: the last tile's V rows past the end, whose probabilities are
+// 0, are cleared (0 x NaN), and rows past the end have no say in when a warp refreshes its maxima.
+template <int DH, int POLY, int EXP, bool PAD, int SPLIT, typename E = __half, bool OP = false>
 __global__ void __launch_bounds__(kThreads3, 2)
     attention_tc3_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_kv,
                          const __grid_constant__ CUtensorMap tmap_qlo, const __grid_constant__ CUtensorMap tmap_klo,
                          const AttnParams p) {
-  static_assert(!PAD || DH == 32, "padded heads use the 32-column tiles");
+  static_assert(!PAD || DH == 32 || OP, "the encoder's padded heads use the 32-column tiles");
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  static_assert(SPLIT == (PAD ? 2 : 0), "the padded heads, and only they, take split scores");
+  static_assert(SPLIT == (PAD && !OP ? 2 : 0), "the encoder's padded heads, and only they, take split scores");
+  static_assert(!OP || (PAD && EXP == 3), "the operator runs on padded maps with the default arithmetic");
   using G = Tc3<DH, SPLIT>;
   constexpr int kD = DH, kQBytes = G::kQBytes, kKVBytes = G::kKVBytes, kOffKV = G::kOffKV;
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + G::kOffBar);
@@ -95,13 +105,23 @@ __global__ void __launch_bounds__(kThreads3, 2)
   uint64_t* step = kv_empty + kStages3;       // [2 tiles][2 buffers]: S and PV completions
   uint64_t* p_full = step + 4;                // [2 tiles][2 buffers]: P written
   uint64_t* drain = p_full + 4;               // [2 tiles]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 2);
+  uint64_t* tail = drain + 2;                 // OP: the last tile has landed
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tail + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int2 wk = p.work[blockIdx.x];
+  int2 wk;
+  if constexpr (OP) wk = make_int2(blockIdx.z, blockIdx.x);
+  else wk = p.work[blockIdx.x];
   const int b = wk.x, q0 = wk.y * (2 * kQ), h = blockIdx.y;
   const int start = p.cu_seqlens[b];
   const int len = p.cu_seqlens[b + 1] - start;
+  if constexpr (OP) {
+    if (!packed_rows(start, len, p.T, p.max_len)) {
+      if (threadIdx.x == 0) atomicOr(p.err, kDevBadSeqlens);
+      return;
+    }
+    if (q0 >= len) return;
+  }
   const int nkv = (len + kKV - 1) / kKV;
   const int ntiles = q0 + kQ < len ? 2 : 1;  // the second query tile holds rows of this sequence
 
@@ -116,6 +136,7 @@ __global__ void __launch_bounds__(kThreads3, 2)
       mbar_init(&p_full[i], 4);
     }
     for (int t = 0; t < 2; ++t) mbar_init(&drain[t], 1);
+    if constexpr (OP) mbar_init(tail, 1);
     fence_mbar_init();
   }
   if (warp == 9) {
@@ -152,6 +173,23 @@ __global__ void __launch_bounds__(kThreads3, 2)
           break;
         }
         uint8_t* dst = smem + kOffKV + st * G::kStageTiles * kKVBytes;
+        const int kept = len - j * kKV;  // keys of this tile inside the sequence
+        if constexpr (OP) {
+          if (kept < kKV) {  // the last tile: its V rows past the end are cleared before it is handed on
+            mbar_arrive_expect_tx(tail, 2 * kKVBytes);
+            tma_load_3d(dst, &tmap_kv, tail, 0, p.H + h, start + j * kKV, pol);
+            tma_load_3d(dst + kKVBytes, &tmap_kv, tail, 0, 2 * p.H + h, start + j * kKV, pol);
+            if (!mbar_wait(tail, 0, p.err, kDevTimeoutProducer)) {
+              ok = false;
+              break;
+            }
+            uint4* v = reinterpret_cast<uint4*>(dst + kKVBytes + kept * kD * 2);  // rows are whole under the swizzle
+            for (int i = 0; i < (kKV - kept) * kD * 2 / 16; ++i) v[i] = make_uint4(0u, 0u, 0u, 0u);
+            fence_proxy_async_smem();
+            mbar_arrive(&kv_full[st]);
+            continue;
+          }
+        }
         mbar_arrive_expect_tx(&kv_full[st], G::kStageTiles * kKVBytes);
         if constexpr (PAD) {
           tma_load_3d(dst, &tmap_kv, &kv_full[st], 0, p.H + h, start + j * kKV, pol);
@@ -179,8 +217,9 @@ __global__ void __launch_bounds__(kThreads3, 2)
     // each issuer (kv_empty counts ntiles arrivals).
     const int t = warp - 9;
     if (t < ntiles && elect_one_sync()) {
-      constexpr uint32_t idesc_qk = umma_idesc_f16(kQ, kKV);
-      constexpr uint32_t idesc_pv = umma_idesc_f16(kQ, kD) | (1u << 16);  // B (V) is MN-major
+      constexpr uint32_t kOperands = std::is_same<E, __half>::value ? 0u : kIdescBf16;
+      constexpr uint32_t idesc_qk = umma_idesc_f16(kQ, kKV) | kOperands;
+      constexpr uint32_t idesc_pv = umma_idesc_f16(kQ, kD) | (1u << 16) | kOperands;  // B (V) is MN-major
       constexpr uint32_t kStageLo = (G::kStageTiles * kKVBytes) >> 4, kVLo = kKVBytes >> 4, kQLo = kQBytes >> 4;
       constexpr uint32_t kVStepLo = (16 * kD * 2) >> 4;  // 16 keys of V
       const uint32_t q_lo = umma_sw128_lo(smem_u32(smem)) + t * kQLo;
@@ -307,8 +346,7 @@ __global__ void __launch_bounds__(kThreads3, 2)
               rs2[i & 3] = f2_add(rs2[i & 3], e2);
               float e0, e1;
               f2_unpack(e2, e0, e1);
-              __half2 hv = __floats2half2_rn(e0, e1);
-              pk[i] = *reinterpret_cast<uint32_t*>(&hv);
+              pk[i] = pack2<E>(e0, e1);
             }
             float r0, r1;
             f2_unpack(f2_add(f2_add(rs2[0], rs2[1]), f2_add(rs2[2], rs2[3])), r0, r1);
@@ -316,7 +354,7 @@ __global__ void __launch_bounds__(kThreads3, 2)
           };
           if (j == 0) mc = max32();
           float ls = exps();
-          if (__any_sync(0xffffffffu, !(ls <= p.rescale_sum))) {
+          if (__any_sync(0xffffffffu, !(ls <= p.rescale_sum) && (!OP || q0 + t * kQ + r < len))) {
             // j >= 1 here: with the exact max of tile 0 every P of step 0 is at most 1.
             load_s();
             const float m_new = fmaxf(mc, max32());
@@ -471,7 +509,9 @@ __global__ void __launch_bounds__(kThreads3, 2)
         const int row = q0 + t * kQ + r;
         const float inv = 1.0f / l;
         const int dh_out = PAD ? p.dh : kD;  // stored columns (the padding is not part of the head)
-        __half* dst = p.out + static_cast<size_t>(start + row) * p.d + h * dh_out;
+        E* dst;
+        if constexpr (OP) dst = static_cast<E*>(p.op_out) + static_cast<size_t>(start + row) * p.ld_out + h * dh_out;
+        else dst = p.out + static_cast<size_t>(start + row) * p.d + h * dh_out;
 #pragma unroll
         for (int hh = 0; hh < kD / 32; ++hh) {
           uint32_t o[32];
@@ -480,12 +520,11 @@ __global__ void __launch_bounds__(kThreads3, 2)
           if (row < len) {
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-              if (PAD && 8 * k >= dh_out) break;
-              __half2 hv[4];
+              if (PAD && hh * 32 + 8 * k >= dh_out) break;
+              uint32_t hv[4];
 #pragma unroll
               for (int e = 0; e < 4; ++e)
-                hv[e] = __floats2half2_rn(__uint_as_float(o[8 * k + 2 * e]) * inv,
-                                          __uint_as_float(o[8 * k + 2 * e + 1]) * inv);
+                hv[e] = pack2<E>(__uint_as_float(o[8 * k + 2 * e]) * inv, __uint_as_float(o[8 * k + 2 * e + 1]) * inv);
               *reinterpret_cast<uint4*>(dst + hh * 32 + 8 * k) = *reinterpret_cast<uint4*>(hv);
             }
           }
@@ -562,6 +601,42 @@ cudaError_t launch_attention_tc3(const CUtensorMap& tm_q, const CUtensorMap& tm_
     case 1: return launch_poly3<64, 1, 0>(tm_q, tm_kv32, tm_qlo, tm_klo, p, s);
     default: return launch_poly3<64, 2, 0>(tm_q, tm_kv32, tm_qlo, tm_klo, p, s);
   }
+}
+
+// The operator runs the same kernel with two eighths of the exponentials on the FP32 pipe, the
+// encoder's measured best.
+template <int DH, typename E>
+cudaError_t launch_op(const CUtensorMap& tm_q, const CUtensorMap& tm_kv, const AttnParams& p, int B, cudaStream_t s) {
+  auto kernel = attention_tc3_kernel<DH, 2, 3, true, 0, E, true>;
+  constexpr int kSmem = Tc3<DH>::kSmem;
+  static std::atomic<unsigned long long> configured{0};
+  cudaError_t e = allow_smem(kernel, kSmem, configured);
+  if (e != cudaSuccess) return e;
+  kernel<<<dim3((p.max_len + 2 * kQ - 1) / (2 * kQ), p.H, B), kThreads3, kSmem, s>>>(tm_q, tm_kv, tm_q, tm_kv, p);
+  return cudaGetLastError();
+}
+
+cudaError_t launch_attention_op(const AttnOp& a, cudaStream_t s) {
+  AttnParams p{};
+  p.op_out = a.out;
+  p.ld_out = a.ld_out;
+  p.lse = a.lse;
+  p.cu_seqlens = a.cu;
+  p.T = a.T;
+  p.max_len = a.max_len;
+  p.H = a.H;
+  p.dh = a.dh;
+  p.scale = a.scale;
+  p.err = a.err;
+  p.rescale_sum = 32768.0f;
+  p.wait_mma_ns = 64;
+  const bool bf16 = a.dtype == ESM_BF16;
+  CUtensorMap tq, tkv;
+  if (!make_tmap_op_heads(&tq, a.qkv, bf16, a.T, 3 * a.H, a.dh, a.ld_qkv, kQ) ||
+      !make_tmap_op_heads(&tkv, a.qkv, bf16, a.T, 3 * a.H, a.dh, a.ld_qkv, kKV))
+    return cudaErrorInvalidValue;
+  if (a.dh <= 32) return bf16 ? launch_op<32, __nv_bfloat16>(tq, tkv, p, a.B, s) : launch_op<32, __half>(tq, tkv, p, a.B, s);
+  return bf16 ? launch_op<64, __nv_bfloat16>(tq, tkv, p, a.B, s) : launch_op<64, __half>(tq, tkv, p, a.B, s);
 }
 
 }  // namespace esm

@@ -251,6 +251,9 @@ __host__ __device__ constexpr uint32_t umma_idesc_f16(int m, int n) {
          (static_cast<uint32_t>(m >> 4) << 24);
 }
 
+// Both operands bf16 instead of f16 (they are of one type in every MMA of these kernels).
+constexpr uint32_t kIdescBf16 = (1u << 7) | (1u << 10);
+
 __device__ __forceinline__ void tmem_alloc(uint32_t* slot_smem, uint32_t ncols) {
   asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot_smem)),
                "r"(ncols)

@@ -1861,7 +1861,7 @@ int check_attention(esm_ctx* c, int32_t type, int32_t B, int32_t T, int32_t max_
   if (B < 0 || T < 0 || max_len < 0 || max_len > T) return fail(c, ESM_EINVAL, "attention: bad B, T or max_len");
   if (H <= 0 || H > 65535 || dh < 8 || dh > 64 || dh % 8)
     return fail(c, ESM_EINVAL, "attention: head_dim must be a multiple of 8 up to 64 and n_heads positive");
-  if (!std::isfinite(scale)) return fail(c, ESM_EINVAL, "attention: scale must be finite");
+  if (!std::isfinite(scale) || !(scale > 0.0f)) return fail(c, ESM_EINVAL, "attention: scale must be positive and finite");
   if (B > 65535) return fail(c, ESM_EINVAL, "attention: more than 65535 sequences");
   return ESM_OK;
 }

@@ -47,6 +47,13 @@ bool make_tmap_f16_box(CUtensorMap* map, const void* base, uint64_t rows, uint64
 bool make_tmap_f16_heads(CUtensorMap* map, const void* base, uint64_t rows, uint64_t heads, uint32_t head_dim,
                          uint64_t ld, uint32_t box_rows);
 
+// Map over the heads of a caller's [rows, ld] matrix of fp16 or bf16 for the attention operators: the
+// 3-D view [rows][heads][head_dim] (head_dim a multiple of 8 up to 64) with boxes of W x 1 x box_rows, W = 32
+// for head_dim up to 32 (64-byte swizzle) and 64 above (128-byte swizzle), zero-padded like
+// make_tmap_f16_heads'.
+bool make_tmap_op_heads(CUtensorMap* map, const void* base, bool bf16, uint64_t rows, uint64_t heads,
+                        uint32_t head_dim, uint64_t ld, uint32_t box_rows);
+
 // Tensor map for the epilogue's bulk stores: a row-major [rows, cols] matrix of fp16 (elem_bytes 2)
 // or fp32 (4), box = [32 rows, 64 bytes], 64-byte swizzle.
 bool make_tmap_out(CUtensorMap* map, const void* base, int elem_bytes, uint64_t rows, uint64_t cols, uint64_t ld);

@@ -90,6 +90,11 @@ struct AttnParams {
   // tcgen05 kernel: suspension hint (ns, 0 = spin) of the MMA issuers' waits, so that the issuers
   // take few issue slots from the softmax warps that share their sub-partitions.
   uint32_t wait_mma_ns;
+  // the attention operator (train_ops.cuh): output of its element type and row stride, and the bound
+  // of the sequences' lengths; out, work, n_work, qkv and d are the encoder's
+  void* op_out;
+  int64_t ld_out;
+  int max_len;
 };
 // mma.sync attention (attention.cu): work items are (sequence, 64-row query tile); any head_dim
 // that is a multiple of 8 up to 64.

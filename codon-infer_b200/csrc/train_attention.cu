@@ -19,13 +19,13 @@ constexpr int kWarps = 8;
 
 // Sequence b of a call, or length 0 where the offsets are not those of packed rows in [0, T].
 __device__ __forceinline__ int sequence(const AttnOp& p, int b, int* start) {
-  const int s0 = p.cu[b], s1 = p.cu[b + 1];
-  *start = s0;
-  if (s0 < 0 || s1 < s0 || s1 > p.T || s1 - s0 > p.max_len) {
+  *start = p.cu[b];
+  const int len = p.cu[b + 1] - *start;
+  if (!packed_rows(*start, len, p.T, p.max_len)) {
     if (threadIdx.x == 0) atomicOr(p.err, kDevBadSeqlens);
     return 0;
   }
-  return s1 - s0;
+  return len;
 }
 
 template <typename E>
@@ -33,36 +33,6 @@ __device__ __forceinline__ float dot_row(const E* a, const E* b, int dh) {
   float s = 0.0f;
   for (int d = 0; d < dh; ++d) s = fmaf(to_f32(a[d]), to_f32(b[d]), s);
   return s;
-}
-
-template <typename E>
-__global__ void attention_op_kernel(const AttnOp p) {
-  int start;
-  const int len = sequence(p, blockIdx.z, &start), h = blockIdx.y, lane = threadIdx.x & 31;
-  const int i = blockIdx.x * kWarps + (threadIdx.x >> 5), dh = p.dh, d = p.H * dh;
-  if (i >= len) return;
-  const E* qkv = static_cast<const E*>(p.qkv);
-  const E* q = qkv + static_cast<size_t>(start + i) * p.ld_qkv + h * dh;
-  float m = -INFINITY, l = 0.0f, acc[2] = {0.0f, 0.0f};
-  for (int j0 = 0; j0 < len; j0 += 32) {
-    const int n = min(32, len - j0);
-    const E* k = qkv + static_cast<size_t>(start + j0 + min(lane, n - 1)) * p.ld_qkv + d + h * dh;
-    const float s = lane < n ? dot_row(q, k, dh) * p.scale : -INFINITY;
-    const float m_new = fmaxf(m, warp_max(s)), a = expf(m - m_new), e = expf(s - m_new);
-    l = l * a + warp_sum(e);
-    m = m_new;
-    for (int c = 0; c < 2; ++c) acc[c] *= a;
-    for (int r = 0; r < n; ++r) {
-      const float pr = __shfl_sync(0xffffffffu, e, r);
-      const E* v = qkv + static_cast<size_t>(start + j0 + r) * p.ld_qkv + 2 * d + h * dh;
-      for (int c = 0; c < 2; ++c)
-        if (lane + 32 * c < dh) acc[c] = fmaf(pr, to_f32(v[lane + 32 * c]), acc[c]);
-    }
-  }
-  E* o = static_cast<E*>(p.out) + static_cast<size_t>(start + i) * p.ld_out + h * dh;
-  for (int c = 0; c < 2; ++c)
-    if (lane + 32 * c < dh) o[lane + 32 * c] = from_f32<E>(acc[c] / l);
-  if (lane == 0 && p.lse) p.lse[static_cast<size_t>(h) * p.T + start + i] = m + logf(l);
 }
 
 // D = rowsum(dO O) into the workspace, [H, T].
@@ -127,13 +97,6 @@ cudaError_t backward(const AttnOp& p, cudaStream_t s) {
 }
 
 }  // namespace
-
-cudaError_t launch_attention_op(const AttnOp& p, cudaStream_t s) {
-  const dim3 grid((p.max_len + kWarps - 1) / kWarps, p.H, p.B);
-  if (p.dtype == ESM_F16) attention_op_kernel<__half><<<grid, kWarps * 32, 0, s>>>(p);
-  else attention_op_kernel<__nv_bfloat16><<<grid, kWarps * 32, 0, s>>>(p);
-  return cudaGetLastError();
-}
 
 size_t attention_backward_bytes(int B, int T, int H) {
   return static_cast<size_t>(H) * T * 4 + static_cast<size_t>(H) * (T / 64 + B) * 8;

@@ -6,6 +6,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/esm_b200.h"
 
 namespace esm {
@@ -21,6 +23,38 @@ template <>
 __device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
+// Two values rounded to E, the first in the low half.
+template <typename E>
+__device__ __forceinline__ uint32_t pack2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+  const __half2 v = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// Whether a sequence's offsets (its first row and its length) are rows of a [T, *] buffer and within
+// the length that the launch was sized for.
+__device__ __forceinline__ bool packed_rows(int start, int len, int T, int max_len) {
+  return start >= 0 && len >= 0 && len <= max_len && start <= T - len;
+}
+
+// Lets a kernel use `bytes` of dynamic shared memory on the current device, once per device.
+template <typename K>
+cudaError_t allow_smem(K kernel, int bytes, std::atomic<unsigned long long>& configured) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 64 && (configured.load(std::memory_order_acquire) & (1ull << dev))) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && dev < 64) configured.fetch_or(1ull << dev, std::memory_order_release);
+  return e;
+}
 
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
