@@ -603,13 +603,33 @@ def test_logprobs_ties_masks_and_rows_without_a_distribution(m, V):
 def test_logprobs_adversarial_order(m):
     """The largest logits at a fixed stride, so that they all fall to the same threads; and sorted rows."""
     V, k = 32768, 64
-    x = randn(31, 4, V)
+    x = randn(31, 8, V)
+    at = torch.arange(V, device="cuda")
+    x[4] += 40.0 * ((at // 4) % 512 < 32)     # one warp's worth of vectors, all far above the rest
+    x[5] = ((at // 4) % 512 < 64).float()     # the same as ties
+    x[6] = (at % 2).float()
+    x[7] += 40.0 * ((at // 4) % 128 < 96)
     x[0, 5::256][:k] += 50
     x[1, ::1024] += 50
     x[2] = torch.linspace(-20, 20, V, device="cuda")
     x[3] = torch.linspace(20, -20, V, device="cuda")
-    targets = torch.zeros(4, dtype=torch.int32, device="cuda")
+    targets = torch.zeros(8, dtype=torch.int32, device="cuda")
     check_logprobs(x, targets, *run_logprobs(m, x, targets, k))
+    for n in (1000, 4000):                    # the smaller blocks
+        y = x[:, :n].contiguous()
+        y[4] = 40.0 * ((at[:n] // 4) % 128 < 32) + randn(32, n)
+        check_logprobs(y, targets, *run_logprobs(m, y, targets, 16))
+        check_logprobs(y, targets, *run_logprobs(m, y, targets, k))
+
+
+def test_logprobs_are_reproducible(m):
+    for V, k in ((33, 8), (700, 9), (4000, 33), (32003, 64)):
+        x = logits_of(64, V, "bf16", seed=V)
+        targets = torch.full((64,), 5, dtype=torch.int32, device="cuda")
+        first = run_logprobs(m, x, targets, k)
+        for _ in range(3):
+            for a, b in zip(first, run_logprobs(m, x, targets, k)):
+                assert torch.equal(a, b)
 
 
 def test_logprobs_row_strides_and_optional_outputs(m, esm):
@@ -736,6 +756,18 @@ def test_distill_rows_without_alternatives_and_padding(m, V):
     want[4] = 0
     want[4:7] -= 1 / 3
     within(dx[7], want, torch.full_like(want, 1e-6), "dlogits of a token ruled out")
+
+
+@pytest.mark.parametrize("V", [33, 300])
+def test_distill_bad_numbers_show(m, V):
+    """A NaN teacher logit of a present alternative, or student logit, is not hidden."""
+    x, ids, top, dloss = distill_inputs(3, V, 2, "f32", seed=46)
+    dloss[:] = 1.0
+    top[0, 1] = math.nan
+    x[1, 7] = math.nan
+    loss, _, dx = run_distill(m, x, ids, top, dloss, 1.0)
+    assert torch.isnan(loss[:2]).all() and torch.isfinite(loss[2])
+    assert torch.isnan(dx[0, ids[0, 1].long()]) and torch.isnan(dx[1]).all() and torch.isfinite(dx[2]).all()
 
 
 def test_distill_row_strides(m):
