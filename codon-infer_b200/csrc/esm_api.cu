@@ -1861,7 +1861,7 @@ int check_attention(esm_ctx* c, int32_t type, int32_t B, int32_t T, int32_t max_
   if (B < 0 || T < 0 || max_len < 0 || max_len > T) return fail(c, ESM_EINVAL, "attention: bad B, T or max_len");
   if (H <= 0 || H > 65535 || dh < 8 || dh > 64 || dh % 8)
     return fail(c, ESM_EINVAL, "attention: head_dim must be a multiple of 8 up to 64 and n_heads positive");
-  if (!std::isfinite(scale) || !(scale > 0.0f)) return fail(c, ESM_EINVAL, "attention: scale must be positive and finite");
+  if (!(scale >= 1e-6f && scale <= 1e6f)) return fail(c, ESM_EINVAL, "attention: scale must be in [1e-6, 1e6]");
   if (B > 65535) return fail(c, ESM_EINVAL, "attention: more than 65535 sequences");
   return ESM_OK;
 }
@@ -1970,6 +1970,7 @@ int esm_attention_backward(esm_ctx* c, int32_t type, const void* d_qkv, int64_t 
   p.dqkv = d_dqkv;
   p.ld_dqkv = ld_dqkv;
   p.workspace = static_cast<float*>(d_workspace);
+  p.num_sms = c->num_sms;
   p.err = c->d_err;
   ESM_CUDA(esm::launch_attention_backward(p, s));
   return ESM_OK;

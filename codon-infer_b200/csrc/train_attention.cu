@@ -4,58 +4,83 @@
 //   dQ = scale dS K,  dK = scale dS^T Q,  dV = P^T dO
 //
 // Two kernels. attention_delta_kernel computes D (and, for fp16, the largest |dO| and |V| of every 64
-// rows). attention_backward_kernel has two kinds of blocks: query blocks own 128 query rows, stream
-// the sequence's keys and values and accumulate dQ; key blocks own 128 keys, stream queries and dO and
-// accumulate dK and dV. So every gradient is summed by one block in a fixed order, without atomics or
-// an fp32 copy of dQ; the price is that S and dO V^T are computed twice (7 products instead of 5).
+// rows). attention_backward_kernel works on items of two kinds: a query item owns 128 query rows,
+// streams the sequence's keys and values and accumulates dQ; a key item owns 128 keys, streams queries
+// and dO and accumulates dK and dV. So every gradient is summed by one block in a fixed order, without
+// atomics or an fp32 copy of dQ; the price is that S and dO V^T are computed twice (7 products, not 5).
 //
-// Both kinds are one scheme. A block owns two 128-row operands A1, A2 and streams 64-row tiles B1, B2:
+// Both kinds are one scheme. An item owns two 128-row operands A1, A2 and streams 64-row tiles B1, B2:
 //               A1   A2   B1   B2
 //   queries     Q    dO   K    V      S = A1 B1^T, dP = A2 B2^T, acc1 (dQ) += dS B1
 //   keys        K    V    Q    dO     S^T = A1 B1^T, dP^T = A2 B2^T, acc1 (dK) += dS^T B1, acc2 (dV) += P^T B2
-// Tensor memory (256 columns, so two blocks fit an SM and one's softmax runs under the other's MMAs):
-// S in [0, 64), dP in [64, 128), acc1 in [128, 192), acc2 in [192, 256). Eight warps do the
-// elementwise work, two per 32-lane quarter, each on 32 of the 64 columns; P and dS go back as 16-bit
-// pairs over the first 16 columns of the same warp's 32 and are read from there as the A operand.
-//   warps 0..7  elementwise: warp w has lanes 32 (w & 3).. and columns 32 (w >> 2)..
-//   warp 8      TMA producer (and, for key blocks, lse and D of the streamed queries)
-//   warp 9      tcgen05.mma issuer
+//
+// One persistent block per SM takes every gridDim.x-th item. Tensor memory (512 columns): three score
+// buffers of 128 columns (S in the first 64, dP in the other 64), acc1 and acc2. Step n uses buffer n % 3 and
+// is worked on by elementwise team n % 2, so the tensor cores compute the next steps' scores and the last
+// one's products meanwhile. P and dS go back over S and dP as 16-bit pairs (each warp over the first half of the
+// 32 columns it read) and are read from there as the A operand.
+//   warps 0..15  elementwise: two teams of eight, a warp has 32 owned rows and 32 of the 64 columns
+//   warps 16..19 store an item's gradients while the teams go on with the next item
+//   warp 20      producer: finds items, loads their operands (two slots) and the stream (TMA ring)
+//   warp 21      tcgen05.mma issuer: S(n + 3) follows the products of step n, which free its buffer
+// Steps, buffers and stages are numbered through all items, so an item's first scores are computed while the
+// one before it is still finishing.
+//
+// In key items lse and D belong to the columns of a thread's row. Reading them for every row costs more
+// shared-memory bandwidth than all operand reads of the tensor cores (a 16-byte broadcast read is four
+// wavefronts), so they are subtracted by the tensor cores: one more K step of 16 with the constants
+// (2^15, 1, 2^-14) in every row of A and -lse / scale, or -D, split into three parts of the operand type
+// in B, which represents fp32 values between about 2^-30 and 2^30 to 2^-24 or better.
+//
 // Heads narrower than 32 or 64 columns arrive zero-padded by the 3-D tensor maps. Rows past the
 // sequence's end in the last streamed tile are cleared in shared memory (they belong to other
 // sequences, and 0 x NaN is not 0); rows past the end of the owned tile stay in their own lanes and
 // are not stored.
 //
-// fp16: P and dS are scaled by powers of two before they are rounded, P by 2^14 in key blocks and dS
+// fp16: P and dS are scaled by powers of two before they are rounded, P by 2^14 in key items and dS
 // by 2^e with 2^e * 2 dh max|dO| max|V| <= 2^14, which bounds it; the outputs are scaled back in fp32.
 #include "common.cuh"
 #include "gemm_tc.cuh"
 #include "train_common.cuh"
 #include "train_ops.cuh"
 
+#include <algorithm>
 #include <type_traits>
 
 namespace esm {
 
 namespace {
 
-constexpr int kOwn = 128;      // rows a block owns
+constexpr int kOwn = 128;      // rows an item owns
 constexpr int kStep = 64;      // rows of a streamed tile
-constexpr int kStages = 4;
-constexpr int kThreads = 320;
+constexpr int kBufs = 3;       // score buffers
+constexpr int kTeams = 2;      // elementwise teams
+constexpr int kTeamWarps = 8;
+constexpr int kStoreWarp = kTeams * kTeamWarps, kLoadWarp = kStoreWarp + 4, kMmaWarp = kLoadWarp + 1;
+constexpr int kThreads = 32 * (kMmaWarp + 1);
+constexpr int kInfos = 8;      // item records: the producer is at most 5 items ahead of the slowest reader
 constexpr int kDeltaRows = 64;
-constexpr uint32_t kTmemCols = 256, kColS = 0, kColDp = 64, kColAcc1 = 128, kColAcc2 = 192;
+constexpr uint32_t kTmemCols = 512, kColBuf = 128, kColDp = 64, kColAcc1 = 384, kColAcc2 = 448;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kPolyEighths = 2;  // exponential pairs of every 8 on the FP32 pipe, as in the forward kernel
 
+struct Item {
+  int start, len, r0, h, keys, ds_exp;  // len 0: no more items
+};
+
 template <int DH>
 struct Bwd {
+  static constexpr int kStages = DH == 64 ? 5 : 8;
   static constexpr int kOwnBytes = kOwn * DH * 2;
   static constexpr int kTileBytes = kStep * DH * 2;
-  static constexpr int kOffStream = 2 * kOwnBytes;
-  static constexpr int kOffStats = kOffStream + kStages * 2 * kTileBytes;  // per stage: 64 lse terms, 64 D terms
-  static constexpr int kOffBar = kOffStats + kStages * 2 * kStep * 4;
-  static constexpr int kSmem = kOffBar + 256 + 1024;
+  static constexpr int kOffConst = 4 * kOwnBytes;                      // two slots of A1, A2
+  static constexpr int kOffStream = kOffConst + kOwnBytes;             // the constants' rows
+  static constexpr int kStageBytes = 3 * kTileBytes;                   // B1, B2, and lse and D in parts
+  static constexpr int kOffInfo = kOffStream + kStages * kStageBytes;
+  static constexpr int kOffBar = kOffInfo + kInfos * 32;
+  static constexpr int kSmem = kOffBar + 512 + 1024;
   static constexpr uint32_t kDescHi = DH == 64 ? kSw128DescHi : kSw64DescHi;
+  static_assert(kSmem <= 232448 && sizeof(Item) <= 32, "shared memory of one block");
 };
 
 struct BwdParams {
@@ -69,7 +94,7 @@ struct BwdParams {
   float* delta;            // [H, T]
   float* peaks;            // fp16: [2][H][blocks], largest |dO| and |V| of each 64 rows
   int blocks;              // T / 64 + B
-  int T, max_len, H, dh;
+  int B, T, max_len, H, dh;
   float scale;
   int* err;
 };
@@ -150,42 +175,97 @@ __device__ __forceinline__ int ds_exponent(const BwdParams& p, int start, int le
   return min(60, max(-60, 13 - ilogbf(bound)));
 }
 
-template <int DH, typename E, bool KEYS>
-__device__ __forceinline__ void backward_block(const CUtensorMap& tm_qkv, const CUtensorMap& tm_dout, const BwdParams& p,
-                                               const int tile) {
+// x as three values of E, times 2^15, 1 and 2^-14 for fp16 (whose range the factors extend) and 1
+// for bf16, packed into the first 16 bytes of a K step (the other elements are zero).
+template <typename E>
+__device__ __forceinline__ uint4 split_parts(float x) {
+  float part[3];
+  if constexpr (std::is_same<E, __half>::value) {
+    constexpr float kScale[3] = {32768.0f, 1.0f, 1.0f / 16384.0f};
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      part[i] = to_f32(from_f32<E>(fminf(fmaxf(x / kScale[i], -60000.0f), 60000.0f)));
+      x -= part[i] * kScale[i];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      part[i] = to_f32(from_f32<E>(x));
+      x -= part[i];
+    }
+  }
+  return make_uint4(pack2<E>(part[0], part[1]), pack2<E>(part[2], 0.0f), 0u, 0u);
+}
+template <typename E>
+__device__ __forceinline__ uint4 split_factors() {
+  if constexpr (std::is_same<E, __half>::value) return make_uint4(pack2<E>(32768.0f, 1.0f), pack2<E>(1.0f / 16384.0f, 0.0f), 0u, 0u);
+  else return make_uint4(pack2<E>(1.0f, 1.0f), pack2<E>(1.0f, 0.0f), 0u, 0u);
+}
+
+// Byte offset of 16-byte chunk `chunk` of row `row` in a tile with rows of DH elements under the
+// tensor maps' swizzle (128 bytes for DH 64, 64 bytes for DH 32).
+template <int DH>
+__device__ __forceinline__ int swizzled(int row, int chunk) {
+  if constexpr (DH == 64) return row * 128 + ((chunk ^ (row & 7)) << 4);
+  else return row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4);
+}
+
+template <int DH, typename E>
+__global__ void __launch_bounds__(kThreads, 1)
+    attention_backward_kernel(const __grid_constant__ CUtensorMap tm_qkv, const __grid_constant__ CUtensorMap tm_dout,
+                              const BwdParams p) {
   using G = Bwd<DH>;
+  constexpr int kStages = G::kStages;
+  constexpr bool kScaled = std::is_same<E, __half>::value;
+  constexpr int kProbExp = kScaled ? 14 : 0;  // key items round 2^kProbExp P
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  auto info_at = [&](int i) -> Item* { return reinterpret_cast<Item*>(smem + G::kOffInfo + (i % kInfos) * 32); };
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + G::kOffBar);
-  uint64_t* own_full = bars;
-  uint64_t* full = own_full + 1;          // [kStages]
-  uint64_t* empty = full + kStages;       // [kStages]
-  uint64_t* scores = empty + kStages;     // S and dP of a step written
-  uint64_t* probs = scores + 1;           // P and dS of a step written
-  uint64_t* done = probs + 1;             // every MMA finished
-  uint64_t* tail = done + 1;              // the last tile has landed
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tail + 1);
+  uint64_t* info_full = bars;                // [kInfos] an item's record
+  uint64_t* own_full = info_full + kInfos;   // [2]
+  uint64_t* own_empty = own_full + 2;        // [2]
+  uint64_t* full = own_empty + 2;            // [kStages]
+  uint64_t* empty = full + kStages;          // [kStages]
+  uint64_t* scores = empty + kStages;        // [kBufs] S and dP written
+  uint64_t* probs = scores + kBufs;          // [kBufs] P and dS written
+  uint64_t* done = probs + kBufs;            // an item's products finished
+  uint64_t* acc_free = done + 1;             // its accumulators read
+  uint64_t* tail = acc_free + 1;             // a sequence's last tile has landed
+  uint64_t* drain = tail + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, h = blockIdx.y, b = blockIdx.z;
-  int start, len;
-  if (!sequence(p, b, &start, &len)) return;
-  const int r0 = tile * kOwn;
-  if (r0 >= len) return;
-  const int steps = (len + kStep - 1) / kStep;
-
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    mbar_init(own_full, 1);
-    for (int s = 0; s < kStages; ++s) {
-      mbar_init(&full[s], KEYS ? 2 : 1);  // the copies, and the lse and D terms
-      mbar_init(&empty[s], 1);
+    for (int i = 0; i < kInfos; ++i) mbar_init(&info_full[i], 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&own_full[i], 1);
+      mbar_init(&own_empty[i], 1);
     }
-    mbar_init(scores, 1);
-    mbar_init(probs, 8);
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&full[i], 2);  // the copies; the producer's own part
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < kBufs; ++i) {
+      mbar_init(&scores[i], 1);
+      mbar_init(&probs[i], kTeamWarps);
+    }
     mbar_init(done, 1);
+    mbar_init(acc_free, 4);
     mbar_init(tail, 1);
+    mbar_init(drain, 1);
     fence_mbar_init();
   }
-  if (warp == 9) {
+  // The constants' rows (K steps 0 and 1), and zeros behind the parts of lse and D.
+  for (int i = threadIdx.x; i < kOwn * 4; i += kThreads)
+    *reinterpret_cast<uint4*>(smem + G::kOffConst + swizzled<DH>(i >> 2, i & 3)) = (i & 1) ? make_uint4(0u, 0u, 0u, 0u) : split_factors<E>();
+  for (int i = threadIdx.x; i < kStages * kStep * 4; i += kThreads) {
+    const int st = i / (kStep * 4), c = i % (kStep * 4);
+    *reinterpret_cast<uint4*>(smem + G::kOffStream + st * G::kStageBytes + 2 * G::kTileBytes + swizzled<DH>(c >> 2, c & 3)) =
+        make_uint4(0u, 0u, 0u, 0u);
+  }
+  fence_proxy_async_smem();
+  if (warp == kMmaWarp) {
     tmem_alloc(tmem_slot, kTmemCols);
     tmem_relinquish();
   }
@@ -193,222 +273,351 @@ __device__ __forceinline__ void backward_block(const CUtensorMap& tm_qkv, const 
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  constexpr bool kScaled = std::is_same<E, __half>::value;
-  constexpr float kProbExp = kScaled && KEYS ? 14.0f : 0.0f;  // P is rounded as 2^kProbExp P
-  const int ds_exp = ds_exponent<E>(p, start, len, b, h, lane);
-  const float f = ldexpf(1.0f, ds_exp - static_cast<int>(kProbExp));  // dS 2^e = (P 2^kProbExp) (dP - D) f
 
-  if (warp == 8) {
+  if (warp == kLoadWarp) {
     // ---------------- producer ----------------
     const uint64_t pol = l2_policy_evict_normal();
-    if (lane == 0) {
-      mbar_arrive_expect_tx(own_full, 2 * G::kOwnBytes);
-      for (int i = 0; i < 2; ++i) {
-        const int row = start + r0 + i * kStep;
-        tma_load_3d(smem + i * G::kTileBytes, &tm_qkv, own_full, 0, KEYS ? p.H + h : h, row, pol);
-        if (KEYS) tma_load_3d(smem + G::kOwnBytes + i * G::kTileBytes, &tm_qkv, own_full, 0, 2 * p.H + h, row, pol);
-        else tma_load_3d(smem + G::kOwnBytes + i * G::kTileBytes, &tm_dout, own_full, 0, h, row, pol);
-      }
-    }
-    const float* lse = p.lse + static_cast<size_t>(h) * p.T + start;
-    const float* delta = p.delta + static_cast<size_t>(h) * p.T + start;
+    const int tiles = (p.max_len + kOwn - 1) / kOwn;
+    const int64_t half = static_cast<int64_t>(tiles) * p.H * p.B, total = 2 * half;
     bool ok = true;
-    int j = 0;
-    for (; j < steps; ++j) {
-      const int st = j % kStages, kept = len - j * kStep;  // rows of this tile inside the sequence
-      if (!mbar_wait(&empty[st], ((j / kStages) & 1) ^ 1u, p.err, kDevTimeoutProducer)) ok = false;
-      if (!__all_sync(0xffffffffu, ok)) break;
-      uint8_t* dst = smem + G::kOffStream + st * 2 * G::kTileBytes;
-      if (lane == 0) {
-        uint64_t* bar = kept < kStep ? tail : &full[st];
-        mbar_arrive_expect_tx(bar, 2 * G::kTileBytes);
-        const int row = start + j * kStep;
-        tma_load_3d(dst, &tm_qkv, bar, 0, KEYS ? h : p.H + h, row, pol);
-        if (KEYS) tma_load_3d(dst + G::kTileBytes, &tm_dout, bar, 0, h, row, pol);
-        else tma_load_3d(dst + G::kTileBytes, &tm_qkv, bar, 0, 2 * p.H + h, row, pol);
+    int item = 0, n = 0, tails = 0;
+    // Loads in flight when a wait gives up must land before the block exits.
+    int own_loaded = 0;
+    for (int64_t base = blockIdx.x; base < total && ok; base += static_cast<int64_t>(32) * gridDim.x) {
+      // 32 candidates at a time, one per lane.
+      const int64_t at = base + static_cast<int64_t>(lane) * gridDim.x;
+      Item it{};
+      int b = 0;
+      if (at < total) {
+        const int64_t r = at < half ? at : at - half;
+        it.keys = at < half;
+        it.r0 = static_cast<int>(r % tiles) * kOwn;
+        it.h = static_cast<int>(r / tiles % p.H);
+        b = static_cast<int>(r / tiles / p.H);
+        it.start = p.cu[b];
+        it.len = p.cu[b + 1] - it.start;
+        if (!packed_rows(it.start, it.len, p.T, p.max_len)) {
+          atomicOr(p.err, kDevBadSeqlens);
+          it.len = 0;
+        }
+        if (it.r0 >= it.len) it.len = 0;
       }
-      if constexpr (KEYS) {
-        float* stats = reinterpret_cast<float*>(smem + G::kOffStats) + st * 2 * kStep;
+      for (uint32_t found = __ballot_sync(0xffffffffu, it.len > 0); found != 0 && ok; found &= found - 1) {
+        const int src = __ffs(found) - 1;
+        Item cur;
+        cur.start = __shfl_sync(0xffffffffu, it.start, src);
+        cur.len = __shfl_sync(0xffffffffu, it.len, src);
+        cur.r0 = __shfl_sync(0xffffffffu, it.r0, src);
+        cur.h = __shfl_sync(0xffffffffu, it.h, src);
+        cur.keys = __shfl_sync(0xffffffffu, it.keys, src);
+        const int cb = __shfl_sync(0xffffffffu, b, src);
+        cur.ds_exp = ds_exponent<E>(p, cur.start, cur.len, cb, cur.h, lane);
+        const int slot = item & 1, h = cur.h, len = cur.len, start = cur.start;
+        const bool keys = cur.keys;
+        ok = mbar_wait_spin(&own_empty[slot], ((item >> 1) & 1) ^ 1u, p.err, kDevTimeoutProducer);
+        if (!__all_sync(0xffffffffu, ok)) {
+          ok = false;
+          break;
+        }
+        if (lane == 0) {
+          *info_at(item) = cur;
+          mbar_arrive(&info_full[item % kInfos]);
+          mbar_arrive_expect_tx(&own_full[slot], 2 * G::kOwnBytes);
+          uint8_t* dst = smem + slot * 2 * G::kOwnBytes;
+          for (int i = 0; i < 2; ++i) {
+            const int row = start + cur.r0 + i * kStep;
+            tma_load_3d(dst + i * G::kTileBytes, &tm_qkv, &own_full[slot], 0, keys ? p.H + h : h, row, pol);
+            tma_load_3d(dst + G::kOwnBytes + i * G::kTileBytes, keys ? &tm_qkv : &tm_dout, &own_full[slot], 0,
+                        keys ? 2 * p.H + h : h, row, pol);
+          }
+        }
+        own_loaded = item + 1;
+        const float* lse = p.lse + static_cast<size_t>(h) * p.T + start;
+        const float* delta = p.delta + static_cast<size_t>(h) * p.T + start;
+        const float inv_scale = 1.0f / p.scale;
+        float next_l[2], next_d[2];  // lse and D of this lane's two rows of the next tile
+        auto stats = [&](int j) {
 #pragma unroll
-        for (int c = lane; c < kStep; c += 32) {
-          const int row = j * kStep + c;
-          stats[c] = row < len ? fmaf(-lse[row], kLog2e, kProbExp) : -INFINITY;  // P = 0 past the end
-          stats[kStep + c] = row < len ? -delta[row] * f : 0.0f;
+          for (int u = 0; u < 2; ++u) {
+            const int row = j * kStep + lane + 32 * u;
+            next_l[u] = row < len ? lse[row] : 0.0f;
+            next_d[u] = row < len ? delta[row] : 0.0f;
+          }
+        };
+        if (keys) stats(0);
+        for (int j = 0; j * kStep < len; ++j, ++n) {
+          const int st = n % kStages, kept = len - j * kStep;  // rows of this tile inside the sequence
+          ok = mbar_wait_spin(&empty[st], ((n / kStages) & 1) ^ 1u, p.err, kDevTimeoutProducer);
+          if (!__all_sync(0xffffffffu, ok)) {
+            ok = false;
+            break;
+          }
+          uint8_t* dst = smem + G::kOffStream + st * G::kStageBytes;
+          if (lane == 0) {
+            uint64_t* bar = kept < kStep ? tail : &full[st];
+            mbar_arrive_expect_tx(bar, 2 * G::kTileBytes);
+            const int row = start + j * kStep;
+            tma_load_3d(dst, &tm_qkv, bar, 0, keys ? h : p.H + h, row, pol);
+            tma_load_3d(dst + G::kTileBytes, keys ? &tm_dout : &tm_qkv, bar, 0, keys ? h : 2 * p.H + h, row, pol);
+          }
+          if (keys) {
+            uint8_t* parts = dst + 2 * G::kTileBytes;
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              const int row = lane + 32 * u;
+              // P = exp2(c (S - lse / scale)), times 2^kProbExp; 0 past the end.
+              const float x = row < kept ? -(next_l[u] - kProbExp * 0.69314718f) * inv_scale : (kScaled ? -1.9e9f : -1e30f);
+              *reinterpret_cast<uint4*>(parts + swizzled<DH>(row, 0)) = split_parts<E>(x);
+              *reinterpret_cast<uint4*>(parts + swizzled<DH>(row, 2)) = split_parts<E>(-next_d[u]);
+            }
+            stats(j + 1);
+          }
+          if (kept < kStep) {
+            ok = mbar_wait_spin(tail, tails & 1, p.err, kDevTimeoutProducer);
+            if (!__all_sync(0xffffffffu, ok)) {
+              ok = false;
+              break;
+            }
+            ++tails;
+            // Rows stay whole under the swizzle.
+            constexpr int kRow = DH * 2 / 16;
+            for (int i = kept * kRow + lane; i < kStep * kRow; i += 32) {
+              reinterpret_cast<uint4*>(dst)[i] = make_uint4(0u, 0u, 0u, 0u);
+              reinterpret_cast<uint4*>(dst + G::kTileBytes)[i] = make_uint4(0u, 0u, 0u, 0u);
+            }
+          }
+          if (keys || kept < kStep) fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(&full[st]);
+            if (kept < kStep) mbar_arrive(&full[st]);
+          }
         }
-      }
-      if (kept < kStep) {
-        if (!mbar_wait(tail, 0, p.err, kDevTimeoutProducer)) ok = false;
-        if (!__all_sync(0xffffffffu, ok)) break;
-        // Rows stay whole under the swizzle.
-        constexpr int kRow = DH * 2 / 16;
-        for (int i = kept * kRow + lane; i < kStep * kRow; i += 32) {
-          reinterpret_cast<uint4*>(dst)[i] = make_uint4(0u, 0u, 0u, 0u);
-          reinterpret_cast<uint4*>(dst + G::kTileBytes)[i] = make_uint4(0u, 0u, 0u, 0u);
-        }
-        fence_proxy_async_smem();
-      }
-      __syncwarp();
-      if (lane == 0) {
-        if (KEYS) mbar_arrive(&full[st]);
-        if (kept < kStep) mbar_arrive(&full[st]);
+        ++item;
       }
     }
-    if (!ok && lane == 0) {  // let the copies in flight land before the block exits
-      mbar_wait(own_full, 0, p.err, kDevTimeoutProducer);
-      for (int i = (j - kStages > 0 ? j - kStages : 0); i < j; ++i)
+    if (ok) {
+      ok = mbar_wait(&own_empty[item & 1], ((item >> 1) & 1) ^ 1u, p.err, kDevTimeoutProducer);  // the record is free
+      if (lane == 0 && ok) {
+        info_at(item)->len = 0;
+        mbar_arrive(&info_full[item % kInfos]);
+      }
+    } else if (lane == 0) {
+      for (int i = own_loaded > 2 ? own_loaded - 2 : 0; i < own_loaded; ++i)
+        mbar_wait(&own_full[i & 1], (i >> 1) & 1, p.err, kDevTimeoutProducer);
+      for (int i = n > kStages ? n - kStages : 0; i < n; ++i)
         mbar_wait(&full[i % kStages], (i / kStages) & 1, p.err, kDevTimeoutProducer);
     }
-  } else if (warp == 9) {
+  } else if (warp == kMmaWarp) {
     // ---------------- MMA issuer ----------------
+    // One thread. An MMA takes 33 to 50 cycles here and few of them queue up, so what the thread does between
+    // them is kept short: addresses, stages and phases are carried along instead of computed.
     if (elect_one_sync()) {
       constexpr uint32_t kOperands = kScaled ? 0u : kIdescBf16;
       constexpr uint32_t idesc_s = umma_idesc_f16(kOwn, kStep) | kOperands;
       constexpr uint32_t idesc_acc = umma_idesc_f16(kOwn, DH) | (1u << 16) | kOperands;  // B is MN-major
-      constexpr uint32_t kTileLo = G::kTileBytes >> 4, kRowsLo = (16 * DH * 2) >> 4;
-      const uint32_t a1 = umma_sw128_lo(smem_u32(smem)), a2 = a1 + (G::kOwnBytes >> 4);
+      constexpr uint32_t kTileLo = G::kTileBytes >> 4, kOwnLo = G::kOwnBytes >> 4, kRowsLo = (16 * DH * 2) >> 4;
+      const uint32_t consts = umma_sw128_lo(smem_u32(smem + G::kOffConst));
       const uint32_t stream = umma_sw128_lo(smem_u32(smem + G::kOffStream));
-      const uint32_t bar_scores = smem_u32(scores), bar_empty = smem_u32(empty);
-      bool ok = mbar_wait_spin(own_full, 0, p.err, kDevTimeoutMma);
-      for (int j = 0; j < steps && ok; ++j) {
-        const int st = j % kStages;
-        if (!mbar_wait_spin(&full[st], (j / kStages) & 1, p.err, kDevTimeoutMma)) {
-          ok = false;
-          break;
+      const uint32_t acc1 = tmem + kColAcc1, acc2 = tmem + kColAcc2;
+      bool ok = true, more = true;
+      // Scores: item, its steps left, kind, slot of its operands, and the step's stage and buffer.
+      int s_item = 0, s_left = 0, s_keys = 0, s_st = 0, s_phase = 0, s_buf = 0;
+      uint32_t s_a = umma_sw128_lo(smem_u32(smem)), s_b = stream, s_d = tmem;
+      int ahead = 0;  // steps whose scores were issued and whose products were not
+      auto issue_scores = [&]() {
+        if (s_left == 0) {
+          if (!(ok = mbar_wait_spin(&info_full[s_item % kInfos], (s_item / kInfos) & 1, p.err, kDevTimeoutMma))) return;
+          const Item* it = info_at(s_item);
+          if (it->len == 0) {
+            more = false;
+            return;
+          }
+          s_left = (it->len + kStep - 1) / kStep;
+          s_keys = it->keys;
+          if (!(ok = mbar_wait_spin(&own_full[s_item & 1], (s_item >> 1) & 1, p.err, kDevTimeoutMma))) return;
         }
+        if (!(ok = mbar_wait_spin(&full[s_st], s_phase, p.err, kDevTimeoutMma))) return;
         tc_fence_after();
-        const uint32_t b1 = stream + st * 2 * kTileLo, b2 = b1 + kTileLo;
 #pragma unroll
-        for (int k = 0; k < DH / 16; ++k) umma_f16_lo<G::kDescHi>(tmem + kColS, a1 + 2 * k, b1 + 2 * k, idesc_s, k);
+        for (int k = 0; k < DH / 16; ++k) umma_f16_lo<G::kDescHi>(s_d, s_a + 2 * k, s_b + 2 * k, idesc_s, k);
+        if (s_keys) umma_f16_lo<G::kDescHi>(s_d, consts, s_b + 2 * kTileLo, idesc_s, 1u);
 #pragma unroll
-        for (int k = 0; k < DH / 16; ++k) umma_f16_lo<G::kDescHi>(tmem + kColDp, a2 + 2 * k, b2 + 2 * k, idesc_s, k);
-        umma_commit_addr(bar_scores);
-        if (!mbar_wait_spin(probs, j & 1, p.err, kDevTimeoutMma)) {
-          ok = false;
-          break;
+        for (int k = 0; k < DH / 16; ++k)
+          umma_f16_lo<G::kDescHi>(s_d + kColDp, s_a + kOwnLo + 2 * k, s_b + kTileLo + 2 * k, idesc_s, k);
+        if (s_keys) umma_f16_lo<G::kDescHi>(s_d + kColDp, consts + 2, s_b + 2 * kTileLo + 2, idesc_s, 1u);
+        umma_commit(&scores[s_buf]);
+        if (--s_left == 0) {
+          umma_commit(&own_empty[s_item & 1]);
+          s_a = (s_item & 1) ? s_a - 2 * kOwnLo : s_a + 2 * kOwnLo;
+          ++s_item;
         }
+        ++ahead;
+        s_b += 3 * kTileLo;
+        if (++s_st == kStages) {
+          s_st = 0;
+          s_phase ^= 1;
+          s_b = stream;
+        }
+        s_d += kColBuf;
+        if (++s_buf == kBufs) {
+          s_buf = 0;
+          s_d = tmem;
+        }
+      };
+      for (int i = 0; i < kBufs && ok && more; ++i) issue_scores();
+      int item = 0, left = 0, keys = 0, st = 0, buf = 0, phase = 0;
+      uint32_t b1 = stream, d = tmem, add = 0;
+      while (ok && ahead > 0) {
+        if (left == 0) {
+          const Item* it = info_at(item);
+          left = (it->len + kStep - 1) / kStep;
+          keys = it->keys;
+          add = 0;
+          if (item > 0 && !(ok = mbar_wait_spin(acc_free, (item - 1) & 1, p.err, kDevTimeoutMma))) break;
+        }
+        if (!(ok = mbar_wait_spin(&probs[buf], phase, p.err, kDevTimeoutMma))) break;
         tc_fence_after();
+        if (keys) {
 #pragma unroll
-        for (int k = 0; k < kStep / 16; ++k) {
-          const uint32_t col = (k >> 1) * 32 + (k & 1) * 8;  // 16 rows of B: 8 columns of pairs
-          if constexpr (KEYS)
-            umma_f16_ts_lo<G::kDescHi>(tmem + kColAcc2, tmem + kColS + col, b2 + k * kRowsLo, idesc_acc, j > 0 || k > 0);
-          umma_f16_ts_lo<G::kDescHi>(tmem + kColAcc1, tmem + kColDp + col, b1 + k * kRowsLo, idesc_acc, j > 0 || k > 0);
+          for (int k = 0; k < kStep / 16; ++k)  // 16 rows of B: 8 columns of pairs
+            umma_f16_ts_lo<G::kDescHi>(acc2, d + 32 * (k >> 1) + 8 * (k & 1), b1 + kTileLo + k * kRowsLo, idesc_acc, k > 0 ? 1u : add);
         }
-        umma_commit_addr(bar_empty + 8 * st);
+#pragma unroll
+        for (int k = 0; k < kStep / 16; ++k)
+          umma_f16_ts_lo<G::kDescHi>(acc1, d + kColDp + 32 * (k >> 1) + 8 * (k & 1), b1 + k * kRowsLo, idesc_acc, k > 0 ? 1u : add);
+        add = 1;
+        umma_commit(&empty[st]);
+        if (--left == 0) {
+          umma_commit(done);
+          ++item;
+        }
+        --ahead;
+        b1 += 3 * kTileLo;
+        if (++st == kStages) {
+          st = 0;
+          b1 = stream;
+        }
+        d += kColBuf;
+        if (++buf == kBufs) {
+          buf = 0;
+          phase ^= 1;
+          d = tmem;
+        }
+        if (more) issue_scores();
       }
-      umma_commit(done);
-      if (!ok) mbar_wait_spin(done, 0, p.err, kDevTimeoutMma);
+      umma_commit(drain);
+      mbar_wait_spin(drain, 0, p.err, kDevTimeoutMma);
+    }
+  } else if (warp >= kStoreWarp) {
+    // ---------------- gradients of finished items: one owned row per thread ----------------
+    const int quarter = warp & 3;
+    const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+    for (int item = 0;; ++item) {
+      if (!mbar_wait(&info_full[item % kInfos], (item / kInfos) & 1, p.err, kDevTimeoutEpilogue)) break;
+      const Item it = *info_at(item);
+      if (it.len == 0) break;
+      const int row = it.r0 + quarter * 32 + lane;
+      const float back_ds = p.scale * ldexpf(1.0f, -it.ds_exp), back_p = ldexpf(1.0f, -kProbExp);
+      E* dst = static_cast<E*>(p.dqkv) + static_cast<size_t>(it.start + row) * p.ld_dqkv;
+      if (!mbar_wait_hint(done, item & 1, p.err, kDevTimeoutEpilogue, 64)) break;
+      tc_fence_after();
+      const int units = (it.keys ? 2 : 1) * (DH / 32);
+      for (int u = 0; u < units; ++u) {  // 32 columns: of dQ, or of dK and then dV
+        const bool dv = u >= DH / 32;
+        const int col = (u % (DH / 32)) * 32;
+        const float back = dv ? back_p : back_ds;
+        uint32_t o[32];
+        tmem_ld32(lanes + (dv ? kColAcc2 : kColAcc1) + col, o);
+        tmem_ld_wait_regs(o);
+        if (u + 1 == units) {  // the accumulators may be written again
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(acc_free);
+        }
+        if (row < it.len) {
+          E* out = dst + ((it.keys ? (dv ? 2 : 1) : 0) * p.H + it.h) * p.dh + col;
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (col + 8 * k < p.dh) {
+              uint32_t v[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                v[i] = pack2<E>(__uint_as_float(o[8 * k + 2 * i]) * back, __uint_as_float(o[8 * k + 2 * i + 1]) * back);
+              *reinterpret_cast<uint4*>(out + 8 * k) = *reinterpret_cast<const uint4*>(v);
+            }
+        }
+      }
     }
   } else {
     // ---------------- elementwise: one owned row per thread, 32 of the 64 columns ----------------
-    const int quarter = warp & 3, half = warp >> 2;
-    const int row = r0 + quarter * 32 + lane;
-    const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
-    const uint32_t t_s = lanes + kColS + 32 * half, t_dp = lanes + kColDp + 32 * half;
+    const int quarter = warp & 3, half = (warp >> 2) & 1, team = warp / kTeamWarps;
+    const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + 32 * half;
     const float c = p.scale * kLog2e;
-    const uint64_t c2 = f2_pack(c, c), f2 = f2_pack(f, f);
-    uint64_t lse2 = 0, delta2 = 0;
-    if constexpr (!KEYS) {
-      const size_t at = static_cast<size_t>(h) * p.T + start + row;
-      const float l = row < len ? -p.lse[at] * kLog2e : 0.0f, d = row < len ? -p.delta[at] * f : 0.0f;
-      lse2 = f2_pack(l, l);
-      delta2 = f2_pack(d, d);
-    }
+    const uint64_t c2 = f2_pack(c, c);
     bool ok = true;
-    for (int j = 0; j < steps; ++j) {
-      if (!mbar_wait_spin(scores, j & 1, p.err, kDevTimeoutEpilogue)) {
-        ok = false;
-        break;
+    int n = 0;  // steps before this item
+    for (int item = 0; ok; ++item) {
+      if (!mbar_wait_spin(&info_full[item % kInfos], (item / kInfos) & 1, p.err, kDevTimeoutEpilogue)) break;
+      const Item it = *info_at(item);
+      if (it.len == 0) break;
+      const int row = it.r0 + quarter * 32 + lane, steps = (it.len + kStep - 1) / kStep;
+      const float f = ldexpf(1.0f, it.keys ? it.ds_exp - kProbExp : it.ds_exp);
+      const uint64_t f2 = f2_pack(f, f);
+      uint64_t lse2 = 0, delta2 = 0;
+      if (!it.keys) {
+        const size_t at = static_cast<size_t>(it.h) * p.T + it.start + row;
+        const float l = row < it.len ? -p.lse[at] * kLog2e : 0.0f, d = row < it.len ? -p.delta[at] * f : 0.0f;
+        lse2 = f2_pack(l, l);
+        delta2 = f2_pack(d, d);
       }
-      tc_fence_after();
-      const int kept = len - j * kStep - 32 * half;  // of this warp's columns
-      const float* stats = reinterpret_cast<const float*>(smem + G::kOffStats) + (j % kStages) * 2 * kStep + 32 * half;
+      for (int j = (n ^ team) & 1; j < steps; j += kTeams) {  // the steps whose number has the team's parity
+        const int buf = (n + j) % kBufs;
+        if (!(ok = mbar_wait_spin(&scores[buf], ((n + j) / kBufs) & 1, p.err, kDevTimeoutEpilogue))) break;
+        tc_fence_after();
+        const uint32_t t_s = lanes + buf * kColBuf, t_dp = t_s + kColDp;
+        const int kept = it.len - j * kStep - 32 * half;  // of this warp's columns
 #pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        uint32_t s[16], dp[16], pr[8], ds[8];
-        tmem_ld16(t_s + 16 * q, s);
-        tmem_ld16(t_dp + 16 * q, dp);
-        tmem_ld_wait();
-        if (!KEYS && kept < 32) {
+        for (int q = 0; q < 2; ++q) {
+          uint32_t s[16], dp[16], pr[8], ds[8];
+          tmem_ld16(t_s + 16 * q, s);
+          tmem_ld16(t_dp + 16 * q, dp);
+          tmem_ld_wait_regs(s, dp);
+          if (!it.keys && kept < 16 * (q + 1)) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (16 * q + i >= kept) s[i] = __float_as_uint(-INFINITY);
-        }
-#pragma unroll
-        for (int i = 0; i < 8; i += 2) {
-          uint64_t l2[2] = {lse2, lse2}, d2[2] = {delta2, delta2};
-          if constexpr (KEYS) {
-            const ulonglong2 l4 = *reinterpret_cast<const ulonglong2*>(stats + 16 * q + 2 * i);
-            const ulonglong2 d4 = *reinterpret_cast<const ulonglong2*>(stats + kStep + 16 * q + 2 * i);
-            l2[0] = l4.x, l2[1] = l4.y, d2[0] = d4.x, d2[1] = d4.y;
+            for (int i = 0; i < 16; ++i)
+              if (16 * q + i >= kept) s[i] = __float_as_uint(-INFINITY);
           }
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const int k = i + u;
+          for (int k = 0; k < 8; ++k) {
+            const uint64_t s2 = f2_pack(__uint_as_float(s[2 * k]), __uint_as_float(s[2 * k + 1]));
+            const uint64_t d2 = f2_pack(__uint_as_float(dp[2 * k]), __uint_as_float(dp[2 * k + 1]));
             float a0, a1, x0, x1;
-            f2_unpack(f2_fma(f2_pack(__uint_as_float(s[2 * k]), __uint_as_float(s[2 * k + 1])), c2, l2[u]), a0, a1);
+            f2_unpack(f2_fma(s2, c2, lse2), a0, a1);
             const uint64_t e2 = k < kPolyEighths ? poly_exp2_x2(fminf(a0, 126.0f), fminf(a1, 126.0f))
                                                  : f2_pack(fast_exp2(a0), fast_exp2(a1));
-            const uint64_t t2 = f2_fma(f2_pack(__uint_as_float(dp[2 * k]), __uint_as_float(dp[2 * k + 1])), f2, d2[u]);
-            f2_unpack(f2_mul(e2, t2), x0, x1);
+            f2_unpack(f2_mul(e2, f2_fma(d2, f2, delta2)), x0, x1);
             ds[k] = pack2<E>(x0, x1);
-            if constexpr (KEYS) {
-              f2_unpack(e2, x0, x1);
-              pr[k] = pack2<E>(x0, x1);
-            }
+            f2_unpack(e2, x0, x1);
+            pr[k] = pack2<E>(x0, x1);
           }
+          if (it.keys) tmem_st8(t_s + 8 * q, pr);
+          tmem_st8(t_dp + 8 * q, ds);
         }
-        tmem_st8(t_dp + 8 * q, ds);
-        if constexpr (KEYS) tmem_st8(t_s + 8 * q, pr);
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&probs[buf]);
       }
-      tmem_st_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(probs);
-    }
-    if (ok && mbar_wait_spin(done, 0, p.err, kDevTimeoutEpilogue)) {
-      tc_fence_after();
-      // Key blocks: half 0 stores dK, half 1 dV. Query blocks: each half stores half of dQ's columns.
-      const float back = KEYS && half == 1 ? ldexpf(1.0f, -static_cast<int>(kProbExp)) : p.scale * ldexpf(1.0f, -ds_exp);
-      const int part = KEYS ? 1 + half : 0;
-      E* dst = static_cast<E*>(p.dqkv) + static_cast<size_t>(start + row) * p.ld_dqkv + (part * p.H + h) * p.dh;
-      constexpr int kCols = KEYS ? DH : DH / 2;
-      const int col0 = KEYS ? 0 : half * kCols;
-      const uint32_t t_acc = lanes + (KEYS && half == 1 ? kColAcc2 : kColAcc1) + col0;
-#pragma unroll
-      for (int cc = 0; cc < kCols; cc += 16) {
-        uint32_t o[16];
-        tmem_ld16(t_acc + cc, o);
-        tmem_ld_wait();
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const int col = col0 + cc + 8 * k;
-          if (row < len && col < p.dh) {
-            uint32_t v[4];
-#pragma unroll
-            for (int u = 0; u < 4; ++u)
-              v[u] = pack2<E>(__uint_as_float(o[8 * k + 2 * u]) * back, __uint_as_float(o[8 * k + 2 * u + 1]) * back);
-            *reinterpret_cast<uint4*>(dst + col) = *reinterpret_cast<const uint4*>(v);
-          }
-        }
-      }
+      n += steps;
     }
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 9) {
+  if (warp == kMmaWarp) {
     tc_fence_after();
     tmem_dealloc(tmem, kTmemCols);
   }
-}
-
-// Even blocks of x own keys, odd ones queries.
-template <int DH, typename E>
-__global__ void __launch_bounds__(kThreads, 2)
-    attention_backward_kernel(const __grid_constant__ CUtensorMap tm_qkv, const __grid_constant__ CUtensorMap tm_dout,
-                              const BwdParams p) {
-  if (blockIdx.x & 1) backward_block<DH, E, false>(tm_qkv, tm_dout, p, blockIdx.x >> 1);
-  else backward_block<DH, E, true>(tm_qkv, tm_dout, p, blockIdx.x >> 1);
 }
 
 template <int DH, typename E>
@@ -422,8 +631,9 @@ cudaError_t backward(const AttnOp& a, const BwdParams& p, cudaStream_t s) {
   cudaError_t e = allow_smem(attention_backward_kernel<DH, E>, Bwd<DH>::kSmem, configured);
   if (e != cudaSuccess) return e;
   attention_delta_kernel<E><<<dim3((a.max_len + kDeltaRows - 1) / kDeltaRows, a.H, a.B), 256, 0, s>>>(p);
+  const int64_t items = static_cast<int64_t>(2) * ((a.max_len + kOwn - 1) / kOwn) * a.H * a.B;
   attention_backward_kernel<DH, E>
-      <<<dim3(2 * ((a.max_len + kOwn - 1) / kOwn), a.H, a.B), kThreads, Bwd<DH>::kSmem, s>>>(tm_qkv, tm_dout, p);
+      <<<static_cast<unsigned>(std::min<int64_t>(items, a.num_sms)), kThreads, Bwd<DH>::kSmem, s>>>(tm_qkv, tm_dout, p);
   return cudaGetLastError();
 }
 
@@ -448,6 +658,7 @@ cudaError_t launch_attention_backward(const AttnOp& a, cudaStream_t s) {
   p.delta = a.workspace;
   p.peaks = a.workspace + static_cast<size_t>(a.H) * a.T;
   p.blocks = a.T / kDeltaRows + a.B;
+  p.B = a.B;
   p.T = a.T;
   p.max_len = a.max_len;
   p.H = a.H;

@@ -26,6 +26,7 @@ struct AttnOp {
   void* dqkv;              // [T, 3 H dh], row stride ld_dqkv
   int64_t ld_dqkv;
   float* workspace;
+  int num_sms;
   int* err;                // device error word
 };
 cudaError_t launch_attention_op(const AttnOp& p, cudaStream_t s);

@@ -273,8 +273,8 @@ enum { ESM_F32 = 0, ESM_F16 = 1, ESM_BF16 = 2 };
  * h * head_dim of each part; d_out [T, H head_dim]; both with rows on 16-byte boundaries. d_cu_seqlens
  * [B + 1] (int32, DEVICE memory): sequence b is rows cu[b] .. cu[b + 1], empty ones allowed; max_len
  * bounds their lengths. T is the number of rows of the buffers: rows behind the last sequence are
- * left as they are. head_dim is a multiple of 8 up to 64, scale positive; B and n_heads
- * are at most 65535. d_lse [H, T] or NULL (the
+ * left as they are. head_dim is a multiple of 8 up to 64, scale in [1e-6, 1e6]; B and
+ * n_heads are at most 65535. d_lse [H, T] or NULL (the
  * backward pass needs it). Scores, sums and outputs are accumulated in fp32, probabilities are rounded to
  * `type` for the product with V. Offsets that do not fit (descending, beyond T or longer than
  * max_len) are noticed on the device: that sequence is skipped and esm_check_device returns

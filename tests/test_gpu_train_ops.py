@@ -200,7 +200,7 @@ def test_attention_sequences_do_not_see_each_other(m, kind, bad):
 @pytest.mark.parametrize("kind", ["f16", "bf16"])
 def test_attention_sharp_and_flat_scores(m, kind):
     H, dh, lens = 2, 64, [300]
-    for sharp, scale in ((40.0, None), (0.01, None), (1.0, 1e-3), (1.0, 0.3)):
+    for sharp, scale in ((40.0, None), (0.01, None), (1.0, 1e-3), (1.0, 0.3), (1.0, 1e-6), (0.001, 100.0)):
         cu, qkv, dout = attention_inputs(lens, H, dh, kind, seed=7, sharp=sharp)
         out, lse = run_forward(m, cu, qkv, H, 300, scale=scale)
         check_forward(cu, qkv, H, out, lse, scale)
@@ -322,7 +322,7 @@ def test_attention_refusals(m, esm):
     refused("max_len", max_len=-1)
     refused("head_dim", H=8, lse=torch.zeros(8, 64, device="cuda"))   # 4 columns
     refused("head_dim", H=32, lse=torch.zeros(32, 64, device="cuda"))  # 1 column
-    for scale in (math.inf, math.nan, 0.0, -0.3):
+    for scale in (math.inf, math.nan, 0.0, -0.3, 1e-7, 1e7):
         refused("scale", scale=scale)
     refused("workspace", code=esm.ESM_ECAPACITY, ws=ws[:16])
     refused("overlap", dqkv=qkv)
