@@ -22,7 +22,9 @@
 //   warps 0..15  elementwise: two teams of eight, a warp has 32 owned rows and 32 of the 64 columns
 //   warps 16..19 store an item's gradients while the teams go on with the next item
 //   warp 20      producer: finds items, loads their operands (two slots) and the stream (TMA ring)
-//   warp 21      tcgen05.mma issuer: S(n + 3) follows the products of step n, which free its buffer
+//   warp 23      splits lse and D of the streamed queries of key items (below)
+//   warp 21      issues the scores' MMAs: those of step n + 3 once the products of step n have freed its buffer
+//   warp 22      issues the products' MMAs
 // Steps, buffers and stages are numbered through all items, so an item's first scores are computed while the
 // one before it is still finishing.
 //
@@ -56,8 +58,9 @@ constexpr int kStep = 64;      // rows of a streamed tile
 constexpr int kBufs = 3;       // score buffers
 constexpr int kTeams = 2;      // elementwise teams
 constexpr int kTeamWarps = 8;
-constexpr int kStoreWarp = kTeams * kTeamWarps, kLoadWarp = kStoreWarp + 4, kMmaWarp = kLoadWarp + 1;
-constexpr int kThreads = 32 * (kMmaWarp + 1);
+constexpr int kStoreWarp = kTeams * kTeamWarps, kLoadWarp = kStoreWarp + 4;
+constexpr int kScoreWarp = kLoadWarp + 1, kProductWarp = kScoreWarp + 1, kSplitWarp = kProductWarp + 1;
+constexpr int kThreads = 32 * (kSplitWarp + 1);
 constexpr int kInfos = 8;      // item records: the producer is at most 5 items ahead of the slowest reader
 constexpr int kDeltaRows = 64;
 constexpr uint32_t kTmemCols = 512, kColBuf = 128, kColDp = 64, kColAcc1 = 384, kColAcc2 = 448;
@@ -76,7 +79,8 @@ struct Bwd {
   static constexpr int kOffConst = 4 * kOwnBytes;                      // two slots of A1, A2
   static constexpr int kOffStream = kOffConst + kOwnBytes;             // the constants' rows
   static constexpr int kStageBytes = 3 * kTileBytes;                   // B1, B2, and lse and D in parts
-  static constexpr int kOffInfo = kOffStream + kStages * kStageBytes;
+  static constexpr int kOffOut = kOffStream + kStages * kStageBytes;   // 32 gradient rows of each storing warp
+  static constexpr int kOffInfo = kOffOut + kOwnBytes;
   static constexpr int kOffBar = kOffInfo + kInfos * 32;
   static constexpr int kSmem = kOffBar + 512 + 1024;
   static constexpr uint32_t kDescHi = DH == 64 ? kSw128DescHi : kSw64DescHi;
@@ -232,8 +236,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* done = probs + kBufs;            // an item's products finished
   uint64_t* acc_free = done + 1;             // its accumulators read
   uint64_t* tail = acc_free + 1;             // a sequence's last tile has landed
-  uint64_t* drain = tail + 1;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  uint64_t* drain = tail + 1;                // [2] everything an issuer issued
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 2);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -243,7 +247,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&own_empty[i], 1);
     }
     for (int i = 0; i < kStages; ++i) {
-      mbar_init(&full[i], 2);  // the copies; the producer's own part
+      mbar_init(&full[i], 2);  // the copies; the parts of lse and D, or for query items the producer again
       mbar_init(&empty[i], 1);
     }
     for (int i = 0; i < kBufs; ++i) {
@@ -253,7 +257,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(done, 1);
     mbar_init(acc_free, 4);
     mbar_init(tail, 1);
-    mbar_init(drain, 1);
+    for (int i = 0; i < 2; ++i) mbar_init(&drain[i], 1);
     fence_mbar_init();
   }
   // The constants' rows (K steps 0 and 1), and zeros behind the parts of lse and D.
@@ -265,7 +269,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         make_uint4(0u, 0u, 0u, 0u);
   }
   fence_proxy_async_smem();
-  if (warp == kMmaWarp) {
+  if (warp == kScoreWarp) {
     tmem_alloc(tmem_slot, kTmemCols);
     tmem_relinquish();
   }
@@ -332,19 +336,6 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         own_loaded = item + 1;
-        const float* lse = p.lse + static_cast<size_t>(h) * p.T + start;
-        const float* delta = p.delta + static_cast<size_t>(h) * p.T + start;
-        const float inv_scale = 1.0f / p.scale;
-        float next_l[2], next_d[2];  // lse and D of this lane's two rows of the next tile
-        auto stats = [&](int j) {
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const int row = j * kStep + lane + 32 * u;
-            next_l[u] = row < len ? lse[row] : 0.0f;
-            next_d[u] = row < len ? delta[row] : 0.0f;
-          }
-        };
-        if (keys) stats(0);
         for (int j = 0; j * kStep < len; ++j, ++n) {
           const int st = n % kStages, kept = len - j * kStep;  // rows of this tile inside the sequence
           ok = mbar_wait_spin(&empty[st], ((n / kStages) & 1) ^ 1u, p.err, kDevTimeoutProducer);
@@ -360,18 +351,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             tma_load_3d(dst, &tm_qkv, bar, 0, keys ? h : p.H + h, row, pol);
             tma_load_3d(dst + G::kTileBytes, keys ? &tm_dout : &tm_qkv, bar, 0, keys ? h : 2 * p.H + h, row, pol);
           }
-          if (keys) {
-            uint8_t* parts = dst + 2 * G::kTileBytes;
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              const int row = lane + 32 * u;
-              // P = exp2(c (S - lse / scale)), times 2^kProbExp; 0 past the end.
-              const float x = row < kept ? -(next_l[u] - kProbExp * 0.69314718f) * inv_scale : (kScaled ? -1.9e9f : -1e30f);
-              *reinterpret_cast<uint4*>(parts + swizzled<DH>(row, 0)) = split_parts<E>(x);
-              *reinterpret_cast<uint4*>(parts + swizzled<DH>(row, 2)) = split_parts<E>(-next_d[u]);
-            }
-            stats(j + 1);
-          }
           if (kept < kStep) {
             ok = mbar_wait_spin(tail, tails & 1, p.err, kDevTimeoutProducer);
             if (!__all_sync(0xffffffffu, ok)) {
@@ -385,13 +364,11 @@ __global__ void __launch_bounds__(kThreads, 1)
               reinterpret_cast<uint4*>(dst)[i] = make_uint4(0u, 0u, 0u, 0u);
               reinterpret_cast<uint4*>(dst + G::kTileBytes)[i] = make_uint4(0u, 0u, 0u, 0u);
             }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&full[st]);
           }
-          if (keys || kept < kStep) fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) {
-            mbar_arrive(&full[st]);
-            if (kept < kStep) mbar_arrive(&full[st]);
-          }
+          if (!keys && lane == 0) mbar_arrive(&full[st]);
         }
         ++item;
       }
@@ -408,145 +385,215 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int i = n > kStages ? n - kStages : 0; i < n; ++i)
         mbar_wait(&full[i % kStages], (i / kStages) & 1, p.err, kDevTimeoutProducer);
     }
-  } else if (warp == kMmaWarp) {
-    // ---------------- MMA issuer ----------------
-    // One thread. An MMA takes 33 to 50 cycles here and few of them queue up, so what the thread does between
-    // them is kept short: addresses, stages and phases are carried along instead of computed.
+  } else if (warp == kScoreWarp) {
+    // ---------------- scores: one thread issues ----------------
+    // The two issuers are separate warps because an MMA's operands stay in the issuing warp's registers until
+    // the tensor core takes it: a warp stalls there, and what it does next (a commit, a wait, the next
+    // addresses) is not hidden. With one issuer for both that cost 490 of 1265 cycles a step.
     if (elect_one_sync()) {
-      constexpr uint32_t kOperands = kScaled ? 0u : kIdescBf16;
-      constexpr uint32_t idesc_s = umma_idesc_f16(kOwn, kStep) | kOperands;
-      constexpr uint32_t idesc_acc = umma_idesc_f16(kOwn, DH) | (1u << 16) | kOperands;  // B is MN-major
-      constexpr uint32_t kTileLo = G::kTileBytes >> 4, kOwnLo = G::kOwnBytes >> 4, kRowsLo = (16 * DH * 2) >> 4;
+      constexpr uint32_t idesc = umma_idesc_f16(kOwn, kStep) | (kScaled ? 0u : kIdescBf16);
+      constexpr uint32_t kTileLo = G::kTileBytes >> 4, kOwnLo = G::kOwnBytes >> 4;
       const uint32_t consts = umma_sw128_lo(smem_u32(smem + G::kOffConst));
       const uint32_t stream = umma_sw128_lo(smem_u32(smem + G::kOffStream));
-      const uint32_t acc1 = tmem + kColAcc1, acc2 = tmem + kColAcc2;
-      bool ok = true, more = true;
-      // Scores: item, its steps left, kind, slot of its operands, and the step's stage and buffer.
-      int s_item = 0, s_left = 0, s_keys = 0, s_st = 0, s_phase = 0, s_buf = 0;
-      uint32_t s_a = umma_sw128_lo(smem_u32(smem)), s_b = stream, s_d = tmem;
-      int ahead = 0;  // steps whose scores were issued and whose products were not
-      auto issue_scores = [&]() {
-        if (s_left == 0) {
-          if (!(ok = mbar_wait_spin(&info_full[s_item % kInfos], (s_item / kInfos) & 1, p.err, kDevTimeoutMma))) return;
-          const Item* it = info_at(s_item);
-          if (it->len == 0) {
-            more = false;
-            return;
+      bool ok = true;
+      int st = 0, phase = 0, buf = 0, n = 0;       // of the step
+      int freed_st = 0, freed_phase = 0;           // of step n - kBufs
+      uint32_t a = umma_sw128_lo(smem_u32(smem)), b = stream, d = tmem;
+      for (int item = 0; ok; ++item) {
+        if (!(ok = mbar_wait_spin(&info_full[item % kInfos], (item / kInfos) & 1, p.err, kDevTimeoutMma))) break;
+        const int len = info_at(item)->len, keys = info_at(item)->keys;
+        if (len == 0) break;
+        if (!(ok = mbar_wait_spin(&own_full[item & 1], (item >> 1) & 1, p.err, kDevTimeoutMma))) break;
+        for (int left = (len + kStep - 1) / kStep; left > 0; --left, ++n) {
+          if (!(ok = mbar_wait_spin(&full[st], phase, p.err, kDevTimeoutMma))) break;
+          if (n >= kBufs) {  // the products of step n - kBufs have read the buffer
+            if (!(ok = mbar_wait_spin(&empty[freed_st], freed_phase, p.err, kDevTimeoutMma))) break;
+            if (++freed_st == kStages) {
+              freed_st = 0;
+              freed_phase ^= 1;
+            }
           }
-          s_left = (it->len + kStep - 1) / kStep;
-          s_keys = it->keys;
-          if (!(ok = mbar_wait_spin(&own_full[s_item & 1], (s_item >> 1) & 1, p.err, kDevTimeoutMma))) return;
-        }
-        if (!(ok = mbar_wait_spin(&full[s_st], s_phase, p.err, kDevTimeoutMma))) return;
-        tc_fence_after();
+          tc_fence_after();
 #pragma unroll
-        for (int k = 0; k < DH / 16; ++k) umma_f16_lo<G::kDescHi>(s_d, s_a + 2 * k, s_b + 2 * k, idesc_s, k);
-        if (s_keys) umma_f16_lo<G::kDescHi>(s_d, consts, s_b + 2 * kTileLo, idesc_s, 1u);
+          for (int k = 0; k < DH / 16; ++k) umma_f16_lo<G::kDescHi>(d, a + 2 * k, b + 2 * k, idesc, k);
+          if (keys) umma_f16_lo<G::kDescHi>(d, consts, b + 2 * kTileLo, idesc, 1u);
 #pragma unroll
-        for (int k = 0; k < DH / 16; ++k)
-          umma_f16_lo<G::kDescHi>(s_d + kColDp, s_a + kOwnLo + 2 * k, s_b + kTileLo + 2 * k, idesc_s, k);
-        if (s_keys) umma_f16_lo<G::kDescHi>(s_d + kColDp, consts + 2, s_b + 2 * kTileLo + 2, idesc_s, 1u);
-        umma_commit(&scores[s_buf]);
-        if (--s_left == 0) {
-          umma_commit(&own_empty[s_item & 1]);
-          s_a = (s_item & 1) ? s_a - 2 * kOwnLo : s_a + 2 * kOwnLo;
-          ++s_item;
+          for (int k = 0; k < DH / 16; ++k) umma_f16_lo<G::kDescHi>(d + kColDp, a + kOwnLo + 2 * k, b + kTileLo + 2 * k, idesc, k);
+          if (keys) umma_f16_lo<G::kDescHi>(d + kColDp, consts + 2, b + 2 * kTileLo + 2, idesc, 1u);
+          umma_commit(&scores[buf]);
+          b += 3 * kTileLo;
+          if (++st == kStages) {
+            st = 0;
+            phase ^= 1;
+            b = stream;
+          }
+          d += kColBuf;
+          if (++buf == kBufs) {
+            buf = 0;
+            d = tmem;
+          }
         }
-        ++ahead;
-        s_b += 3 * kTileLo;
-        if (++s_st == kStages) {
-          s_st = 0;
-          s_phase ^= 1;
-          s_b = stream;
+        umma_commit(&own_empty[item & 1]);
+        a = (item & 1) ? a - 2 * kOwnLo : a + 2 * kOwnLo;
+      }
+      umma_commit(&drain[0]);
+      mbar_wait_spin(&drain[0], 0, p.err, kDevTimeoutMma);
+    }
+  } else if (warp == kProductWarp) {
+    // ---------------- products: one thread issues ----------------
+    if (elect_one_sync()) {
+      constexpr uint32_t idesc = umma_idesc_f16(kOwn, DH) | (1u << 16) | (kScaled ? 0u : kIdescBf16);  // B is MN-major
+      constexpr uint32_t kTileLo = G::kTileBytes >> 4, kRowsLo = (16 * DH * 2) >> 4;
+      const uint32_t stream = umma_sw128_lo(smem_u32(smem + G::kOffStream));
+      const uint32_t acc1 = tmem + kColAcc1, acc2 = tmem + kColAcc2;
+      bool ok = true;
+      int st = 0, buf = 0, phase = 0;
+      uint32_t b = stream, d = tmem;
+      for (int item = 0; ok; ++item) {
+        if (!(ok = mbar_wait_spin(&info_full[item % kInfos], (item / kInfos) & 1, p.err, kDevTimeoutMma))) break;
+        const int len = info_at(item)->len, keys = info_at(item)->keys;
+        if (len == 0) break;
+        if (item > 0 && !(ok = mbar_wait_spin(acc_free, (item - 1) & 1, p.err, kDevTimeoutMma))) break;
+        uint32_t add = 0;
+        for (int left = (len + kStep - 1) / kStep; left > 0; --left) {
+          if (!(ok = mbar_wait_spin(&probs[buf], phase, p.err, kDevTimeoutMma))) break;
+          tc_fence_after();
+          if (keys) {
+#pragma unroll
+            for (int k = 0; k < kStep / 16; ++k)  // 16 rows of B: 8 columns of pairs
+              umma_f16_ts_lo<G::kDescHi>(acc2, d + 32 * (k >> 1) + 8 * (k & 1), b + kTileLo + k * kRowsLo, idesc, k > 0 ? 1u : add);
+          }
+#pragma unroll
+          for (int k = 0; k < kStep / 16; ++k)
+            umma_f16_ts_lo<G::kDescHi>(acc1, d + kColDp + 32 * (k >> 1) + 8 * (k & 1), b + k * kRowsLo, idesc, k > 0 ? 1u : add);
+          add = 1;
+          umma_commit(&empty[st]);
+          b += 3 * kTileLo;
+          if (++st == kStages) {
+            st = 0;
+            b = stream;
+          }
+          d += kColBuf;
+          if (++buf == kBufs) {
+            buf = 0;
+            phase ^= 1;
+            d = tmem;
+          }
         }
-        s_d += kColBuf;
-        if (++s_buf == kBufs) {
-          s_buf = 0;
-          s_d = tmem;
+        umma_commit(done);
+      }
+      umma_commit(&drain[1]);
+      mbar_wait_spin(&drain[1], 0, p.err, kDevTimeoutMma);
+    }
+  } else if (warp == kSplitWarp) {
+    // ---------------- parts of lse and D of the streamed queries (key items) ----------------
+    const float inv_scale = 1.0f / p.scale;
+    bool ok = true;
+    int st = 0, phase = 1;  // the stage's turn, and the parity of its release before that
+    for (int item = 0; ok; ++item) {
+      if (!mbar_wait_spin(&info_full[item % kInfos], (item / kInfos) & 1, p.err, kDevTimeoutProducer)) break;
+      const Item it = *info_at(item);
+      if (it.len == 0) break;
+      const float* lse = p.lse + static_cast<size_t>(it.h) * p.T + it.start;
+      const float* delta = p.delta + static_cast<size_t>(it.h) * p.T + it.start;
+      float next_l[2], next_d[2];  // of this lane's two rows of the next tile
+      auto stats = [&](int j) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int row = j * kStep + lane + 32 * u;
+          next_l[u] = row < it.len ? lse[row] : 0.0f;
+          next_d[u] = row < it.len ? delta[row] : 0.0f;
         }
       };
-      for (int i = 0; i < kBufs && ok && more; ++i) issue_scores();
-      int item = 0, left = 0, keys = 0, st = 0, buf = 0, phase = 0;
-      uint32_t b1 = stream, d = tmem, add = 0;
-      while (ok && ahead > 0) {
-        if (left == 0) {
-          const Item* it = info_at(item);
-          left = (it->len + kStep - 1) / kStep;
-          keys = it->keys;
-          add = 0;
-          if (item > 0 && !(ok = mbar_wait_spin(acc_free, (item - 1) & 1, p.err, kDevTimeoutMma))) break;
-        }
-        if (!(ok = mbar_wait_spin(&probs[buf], phase, p.err, kDevTimeoutMma))) break;
-        tc_fence_after();
-        if (keys) {
+      if (it.keys) stats(0);
+      for (int j = 0; j * kStep < it.len; ++j) {
+        if (it.keys) {
+          uint4 part_l[2], part_d[2];
 #pragma unroll
-          for (int k = 0; k < kStep / 16; ++k)  // 16 rows of B: 8 columns of pairs
-            umma_f16_ts_lo<G::kDescHi>(acc2, d + 32 * (k >> 1) + 8 * (k & 1), b1 + kTileLo + k * kRowsLo, idesc_acc, k > 0 ? 1u : add);
-        }
+          for (int u = 0; u < 2; ++u) {
+            // P = exp2(c (S - lse / scale)), times 2^kProbExp; 0 past the end.
+            const float x = j * kStep + lane + 32 * u < it.len ? -(next_l[u] - kProbExp * 0.69314718f) * inv_scale : (kScaled ? -1.9e9f : -1e30f);
+            part_l[u] = split_parts<E>(x);
+            part_d[u] = split_parts<E>(-next_d[u]);
+          }
+          stats(j + 1);
+          ok = __all_sync(0xffffffffu, mbar_wait_spin(&empty[st], phase, p.err, kDevTimeoutProducer));
+          if (!ok) break;
+          uint8_t* parts = smem + G::kOffStream + st * G::kStageBytes + 2 * G::kTileBytes;
 #pragma unroll
-        for (int k = 0; k < kStep / 16; ++k)
-          umma_f16_ts_lo<G::kDescHi>(acc1, d + kColDp + 32 * (k >> 1) + 8 * (k & 1), b1 + k * kRowsLo, idesc_acc, k > 0 ? 1u : add);
-        add = 1;
-        umma_commit(&empty[st]);
-        if (--left == 0) {
-          umma_commit(done);
-          ++item;
+          for (int u = 0; u < 2; ++u) {
+            *reinterpret_cast<uint4*>(parts + swizzled<DH>(lane + 32 * u, 0)) = part_l[u];
+            *reinterpret_cast<uint4*>(parts + swizzled<DH>(lane + 32 * u, 2)) = part_d[u];
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&full[st]);
         }
-        --ahead;
-        b1 += 3 * kTileLo;
         if (++st == kStages) {
           st = 0;
-          b1 = stream;
-        }
-        d += kColBuf;
-        if (++buf == kBufs) {
-          buf = 0;
           phase ^= 1;
-          d = tmem;
         }
-        if (more) issue_scores();
       }
-      umma_commit(drain);
-      mbar_wait_spin(drain, 0, p.err, kDevTimeoutMma);
     }
   } else if (warp >= kStoreWarp) {
     // ---------------- gradients of finished items: one owned row per thread ----------------
+    // Rounded rows go through shared memory, so that whole rows are written by neighbouring lanes.
     const int quarter = warp & 3;
     const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+    uint8_t* stage = smem + G::kOffOut + quarter * 32 * DH * 2;
+    constexpr int kChunks = DH / 8;  // 16-byte pieces of a row
     for (int item = 0;; ++item) {
       if (!mbar_wait(&info_full[item % kInfos], (item / kInfos) & 1, p.err, kDevTimeoutEpilogue)) break;
       const Item it = *info_at(item);
       if (it.len == 0) break;
-      const int row = it.r0 + quarter * 32 + lane;
       const float back_ds = p.scale * ldexpf(1.0f, -it.ds_exp), back_p = ldexpf(1.0f, -kProbExp);
-      E* dst = static_cast<E*>(p.dqkv) + static_cast<size_t>(it.start + row) * p.ld_dqkv;
       if (!mbar_wait_hint(done, item & 1, p.err, kDevTimeoutEpilogue, 64)) break;
       tc_fence_after();
-      const int units = (it.keys ? 2 : 1) * (DH / 32);
-      for (int u = 0; u < units; ++u) {  // 32 columns: of dQ, or of dK and then dV
-        const bool dv = u >= DH / 32;
-        const int col = (u % (DH / 32)) * 32;
-        const float back = dv ? back_p : back_ds;
-        uint32_t o[32];
-        tmem_ld32(lanes + (dv ? kColAcc2 : kColAcc1) + col, o);
-        tmem_ld_wait_regs(o);
-        if (u + 1 == units) {  // the accumulators may be written again
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(acc_free);
-        }
-        if (row < it.len) {
-          E* out = dst + ((it.keys ? (dv ? 2 : 1) : 0) * p.H + it.h) * p.dh + col;
+      uint32_t v[DH / 2];
+      auto read = [&](uint32_t col, float back) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            if (col + 8 * k < p.dh) {
-              uint32_t v[4];
+        for (int cc = 0; cc < DH / 32; ++cc) {
+          uint32_t o[32];
+          tmem_ld32(lanes + col + 32 * cc, o);
+          tmem_ld_wait_regs(o);
 #pragma unroll
-              for (int i = 0; i < 4; ++i)
-                v[i] = pack2<E>(__uint_as_float(o[8 * k + 2 * i]) * back, __uint_as_float(o[8 * k + 2 * i + 1]) * back);
-              *reinterpret_cast<uint4*>(out + 8 * k) = *reinterpret_cast<const uint4*>(v);
-            }
+          for (int i = 0; i < 16; ++i)
+            v[16 * cc + i] = pack2<E>(__uint_as_float(o[2 * i]) * back, __uint_as_float(o[2 * i + 1]) * back);
         }
+      };
+      auto release = [&]() {  // the accumulators may be written again
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(acc_free);
+      };
+      auto put = [&]() {
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c)
+          *reinterpret_cast<uint4*>(stage + swizzled<DH>(lane, c)) = make_uint4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+        __syncwarp();
+      };
+      auto write = [&](int part) {
+        E* dst = static_cast<E*>(p.dqkv) + (static_cast<size_t>(part) * p.H + it.h) * p.dh;
+#pragma unroll
+        for (int i = 0; i < kChunks; ++i) {
+          const int r = (32 / kChunks) * i + lane / kChunks, c = lane % kChunks, row = it.r0 + quarter * 32 + r;
+          if (row < it.len && 8 * c < p.dh)
+            *reinterpret_cast<uint4*>(dst + static_cast<size_t>(it.start + row) * p.ld_dqkv + 8 * c) =
+                *reinterpret_cast<const uint4*>(stage + swizzled<DH>(r, c));
+        }
+        __syncwarp();
+      };
+      read(kColAcc1, back_ds);
+      if (!it.keys) release();
+      put();
+      if (it.keys) {
+        read(kColAcc2, back_p);
+        release();
+        write(1);
+        put();
+        write(2);
+      } else {
+        write(0);
       }
     }
   } else {
@@ -614,7 +661,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == kMmaWarp) {
+  if (warp == kScoreWarp) {
     tc_fence_after();
     tmem_dealloc(tmem, kTmemCols);
   }
