@@ -15,12 +15,12 @@
 //   keys        K    V    Q    dO     S^T = A1 B1^T, dP^T = A2 B2^T, acc1 (dK) += dS^T B1, acc2 (dV) += P^T B2
 //
 // One persistent block per SM takes every gridDim.x-th item. Tensor memory (512 columns): three score
-// buffers of 128 columns (S in the first 64, dP in the other 64), acc1 and acc2. Step n uses buffer n % 3 and
-// is worked on by elementwise team n % 2, so the tensor cores compute the next steps' scores and the last
-// one's products meanwhile. P and dS go back over S and dP as 16-bit pairs (each warp over the first half of the
-// 32 columns it read) and are read from there as the A operand.
-//   warps 0..15  elementwise: two teams of eight, a warp has 32 owned rows and 32 of the 64 columns
-//   warps 16..19 store an item's gradients while the teams go on with the next item
+// buffers of 128 columns (S in the first 64, dP in the other 64), acc1 and acc2. Step n uses buffer n % 3, so
+// the tensor cores compute the next steps' scores and the last one's products while the elementwise warps
+// work on a step. P and dS go back over S and dP as 16-bit pairs (each warp over the first half of the 16
+// columns it read) and are read from there as the A operand.
+//   warps 0..15  elementwise: a warp has 32 owned rows and 16 of the 64 columns of every step
+//   warps 16..19 store an item's gradients while the others go on with the next item
 //   warp 20      producer: finds items, loads their operands (two slots) and the stream (TMA ring)
 //   warp 23      splits lse and D of the streamed queries of key items (below)
 //   warp 21      issues the scores' MMAs: those of step n + 3 once the products of step n have freed its buffer
@@ -56,16 +56,15 @@ namespace {
 constexpr int kOwn = 128;      // rows an item owns
 constexpr int kStep = 64;      // rows of a streamed tile
 constexpr int kBufs = 3;       // score buffers
-constexpr int kTeams = 2;      // elementwise teams
-constexpr int kTeamWarps = 8;
-constexpr int kStoreWarp = kTeams * kTeamWarps, kLoadWarp = kStoreWarp + 4;
+constexpr int kElemWarps = 16, kTeams = 1, kTeamWarps = kElemWarps / kTeams;
+constexpr int kWarpCols = 4 * kStep / kTeamWarps;  // columns of an elementwise warp
+constexpr int kStoreWarp = kElemWarps, kLoadWarp = kStoreWarp + 4;
 constexpr int kScoreWarp = kLoadWarp + 1, kProductWarp = kScoreWarp + 1, kSplitWarp = kProductWarp + 1;
 constexpr int kThreads = 32 * (kSplitWarp + 1);
 constexpr int kInfos = 8;      // item records: the producer is at most 5 items ahead of the slowest reader
 constexpr int kDeltaRows = 64;
 constexpr uint32_t kTmemCols = 512, kColBuf = 128, kColDp = 64, kColAcc1 = 384, kColAcc2 = 448;
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kPolyEighths = 2;  // exponential pairs of every 8 on the FP32 pipe, as in the forward kernel
 
 struct Item {
   int start, len, r0, h, keys, ds_exp;  // len 0: no more items
@@ -205,6 +204,10 @@ __device__ __forceinline__ uint4 split_factors() {
   if constexpr (std::is_same<E, __half>::value) return make_uint4(pack2<E>(32768.0f, 1.0f), pack2<E>(1.0f / 16384.0f, 0.0f), 0u, 0u);
   else return make_uint4(pack2<E>(1.0f, 1.0f), pack2<E>(1.0f, 0.0f), 0u, 0u);
 }
+
+// Column of the pair of values i, i + 1 of a row of P or dS: every warp packs its columns into the first
+// half of their place.
+__host__ __device__ constexpr int pair_col(int i) { return i / kWarpCols * kWarpCols + i % kWarpCols / 2; }
 
 // Byte offset of 16-byte chunk `chunk` of row `row` in a tile with rows of DH elements under the
 // tensor maps' swizzle (128 bytes for DH 64, 64 bytes for DH 32).
@@ -460,12 +463,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           tc_fence_after();
           if (keys) {
 #pragma unroll
-            for (int k = 0; k < kStep / 16; ++k)  // 16 rows of B: 8 columns of pairs
-              umma_f16_ts_lo<G::kDescHi>(acc2, d + 32 * (k >> 1) + 8 * (k & 1), b + kTileLo + k * kRowsLo, idesc, k > 0 ? 1u : add);
+            for (int k = 0; k < kStep / 16; ++k)  // 16 rows of B: the 8 columns of one warp's pairs
+              umma_f16_ts_lo<G::kDescHi>(acc2, d + pair_col(16 * k), b + kTileLo + k * kRowsLo, idesc, k > 0 ? 1u : add);
           }
 #pragma unroll
           for (int k = 0; k < kStep / 16; ++k)
-            umma_f16_ts_lo<G::kDescHi>(acc1, d + kColDp + 32 * (k >> 1) + 8 * (k & 1), b + k * kRowsLo, idesc, k > 0 ? 1u : add);
+            umma_f16_ts_lo<G::kDescHi>(acc1, d + kColDp + pair_col(16 * k), b + k * kRowsLo, idesc, k > 0 ? 1u : add);
           add = 1;
           umma_commit(&empty[st]);
           b += 3 * kTileLo;
@@ -552,13 +555,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t v[DH / 2];
       auto read = [&](uint32_t col, float back) {
 #pragma unroll
-        for (int cc = 0; cc < DH / 32; ++cc) {
-          uint32_t o[32];
-          tmem_ld32(lanes + col + 32 * cc, o);
-          tmem_ld_wait_regs(o);
+        for (int cc = 0; cc < DH / 16; ++cc) {
+          uint32_t o[16];
+          tmem_ld16(lanes + col + 16 * cc, o);
+          tmem_ld_wait();
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            v[16 * cc + i] = pack2<E>(__uint_as_float(o[2 * i]) * back, __uint_as_float(o[2 * i + 1]) * back);
+          for (int i = 0; i < 8; ++i)
+            v[8 * cc + i] = pack2<E>(__uint_as_float(o[2 * i]) * back, __uint_as_float(o[2 * i + 1]) * back);
         }
       };
       auto release = [&]() {  // the accumulators may be written again
@@ -597,40 +600,52 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
   } else {
-    // ---------------- elementwise: one owned row per thread, 32 of the 64 columns ----------------
-    const int quarter = warp & 3, half = (warp >> 2) & 1, team = warp / kTeamWarps;
-    const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + 32 * half;
+    // ---------------- elementwise: one owned row per thread, 16 of the 64 columns ----------------
+    // All 16 warps share every step: a step's latency from its scores to its products bounds the loop (three
+    // are in flight), not the special-function unit, which takes 512 cycles a step for the exponentials.
+    const int quarter = warp & 3, team = warp / kTeamWarps, cols = kWarpCols * (warp % kTeamWarps >> 2);
+    const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + cols;
     const float c = p.scale * kLog2e;
     const uint64_t c2 = f2_pack(c, c);
-    bool ok = true;
-    int n = 0;  // steps before this item
-    for (int item = 0; ok; ++item) {
-      if (!mbar_wait_spin(&info_full[item % kInfos], (item / kInfos) & 1, p.err, kDevTimeoutEpilogue)) break;
-      const Item it = *info_at(item);
-      if (it.len == 0) break;
-      const int row = it.r0 + quarter * 32 + lane, steps = (it.len + kStep - 1) / kStep;
-      const float f = ldexpf(1.0f, it.keys ? it.ds_exp - kProbExp : it.ds_exp);
-      const uint64_t f2 = f2_pack(f, f);
-      uint64_t lse2 = 0, delta2 = 0;
-      if (!it.keys) {
+    // The record of an item and, for query items, lse and D of this thread's row, which are loaded one step
+    // before they are used.
+    Item it{};
+    float row_l = 0.0f, row_d = 0.0f;
+    auto fetch = [&](int item) {
+      if (!mbar_wait_spin(&info_full[item % kInfos], (item / kInfos) & 1, p.err, kDevTimeoutEpilogue)) return false;
+      it = *info_at(item);
+      const int row = it.r0 + quarter * 32 + lane;
+      if (it.len > 0 && !it.keys && row < it.len) {
         const size_t at = static_cast<size_t>(it.h) * p.T + it.start + row;
-        const float l = row < it.len ? -p.lse[at] * kLog2e : 0.0f, d = row < it.len ? -p.delta[at] * f : 0.0f;
-        lse2 = f2_pack(l, l);
-        delta2 = f2_pack(d, d);
+        row_l = p.lse[at];
+        row_d = p.delta[at];
       }
-      for (int j = (n ^ team) & 1; j < steps; j += kTeams) {  // the steps whose number has the team's parity
-        const int buf = (n + j) % kBufs;
-        if (!(ok = mbar_wait_spin(&scores[buf], ((n + j) / kBufs) & 1, p.err, kDevTimeoutEpilogue))) break;
+      return true;
+    };
+    bool ok = fetch(0);
+    int buf = team % kBufs, phase = 0, skip = team;  // this team's next step: its buffer, and how many steps away
+    for (int item = 0; ok && it.len > 0;) {
+      const bool keys = it.keys;
+      const int len = it.len;
+      const float f = __int_as_float((127 + it.ds_exp - (keys ? kProbExp : 0)) << 23);  // 2^e, or 2^(e - kProbExp)
+      const uint64_t f2 = f2_pack(f, f);
+      const float l = keys ? 0.0f : -row_l * kLog2e, d = keys ? 0.0f : -row_d * f;
+      const uint64_t lse2 = f2_pack(l, l), delta2 = f2_pack(d, d);
+      int left = (len + kStep - 1) / kStep - skip, kept = len - skip * kStep - cols;  // from this warp's first column on
+      ++item;
+      if (left <= 0 && !(ok = fetch(item))) break;
+      for (; left > 0; left -= kTeams, kept -= kTeams * kStep) {
+        if (left <= kTeams && !(ok = fetch(item))) break;
+        if (!(ok = mbar_wait_spin(&scores[buf], phase, p.err, kDevTimeoutEpilogue))) break;
         tc_fence_after();
         const uint32_t t_s = lanes + buf * kColBuf, t_dp = t_s + kColDp;
-        const int kept = it.len - j * kStep - 32 * half;  // of this warp's columns
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
+        for (int q = 0; q < kWarpCols / 16; ++q) {
           uint32_t s[16], dp[16], pr[8], ds[8];
           tmem_ld16(t_s + 16 * q, s);
           tmem_ld16(t_dp + 16 * q, dp);
           tmem_ld_wait_regs(s, dp);
-          if (!it.keys && kept < 16 * (q + 1)) {
+          if (!keys && kept < 16 * (q + 1)) {
 #pragma unroll
             for (int i = 0; i < 16; ++i)
               if (16 * q + i >= kept) s[i] = __float_as_uint(-INFINITY);
@@ -641,22 +656,26 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint64_t d2 = f2_pack(__uint_as_float(dp[2 * k]), __uint_as_float(dp[2 * k + 1]));
             float a0, a1, x0, x1;
             f2_unpack(f2_fma(s2, c2, lse2), a0, a1);
-            const uint64_t e2 = k < kPolyEighths ? poly_exp2_x2(fminf(a0, 126.0f), fminf(a1, 126.0f))
-                                                 : f2_pack(fast_exp2(a0), fast_exp2(a1));
+            const uint64_t e2 = f2_pack(fast_exp2(a0), fast_exp2(a1));
             f2_unpack(f2_mul(e2, f2_fma(d2, f2, delta2)), x0, x1);
             ds[k] = pack2<E>(x0, x1);
             f2_unpack(e2, x0, x1);
             pr[k] = pack2<E>(x0, x1);
           }
-          if (it.keys) tmem_st8(t_s + 8 * q, pr);
+          if (keys) tmem_st8(t_s + 8 * q, pr);
           tmem_st8(t_dp + 8 * q, ds);
         }
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&probs[buf]);
+        buf += kTeams;
+        if (buf >= kBufs) {
+          buf -= kBufs;
+          phase ^= 1;
+        }
       }
-      n += steps;
+      skip = -left;
     }
   }
   tc_fence_before();
