@@ -336,7 +336,15 @@ __device__ __forceinline__ void tmem_ld_wait_regs(uint32_t (&r)[32]) {
                : "memory");
 }
 
-// The same for two loads of 16 columns.
+// The same for one and for two loads of 16 columns.
+__device__ __forceinline__ void tmem_ld_wait_regs(uint32_t (&a)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(a[0]), "+r"(a[1]), "+r"(a[2]), "+r"(a[3]), "+r"(a[4]), "+r"(a[5]), "+r"(a[6]), "+r"(a[7]),
+                 "+r"(a[8]), "+r"(a[9]), "+r"(a[10]), "+r"(a[11]), "+r"(a[12]), "+r"(a[13]), "+r"(a[14]),
+                 "+r"(a[15])
+               :
+               : "memory");
+}
 __device__ __forceinline__ void tmem_ld_wait_regs(uint32_t (&a)[16], uint32_t (&b)[16]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;"
                : "+r"(a[0]), "+r"(a[1]), "+r"(a[2]), "+r"(a[3]), "+r"(a[4]), "+r"(a[5]), "+r"(a[6]), "+r"(a[7]),
@@ -471,6 +479,8 @@ __device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, ui
 constexpr uint32_t kSw128DescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
 // The 64-byte-swizzle layouts (SBO 512 bytes, layout type 4) share the same low-word form.
 constexpr uint32_t kSw64DescHi = (512u >> 4) | (1u << 14) | (4u << 29);
+// K-major rows of one K step (32 bytes) with the 32-byte swizzle (8-row groups 256 bytes apart).
+constexpr uint32_t kSw32DescHi = (256u >> 4) | (1u << 14) | (6u << 29);
 __device__ __forceinline__ uint32_t umma_sw128_lo(uint32_t saddr) { return ((saddr & 0x3FFFFu) >> 4) | (1u << 16); }
 template <uint32_t HI = kSw128DescHi>
 __device__ __forceinline__ void umma_f16_lo(uint32_t tmem_d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc,

@@ -22,7 +22,8 @@
 //   warps 0..15  elementwise: a warp has 32 owned rows and 16 of the 64 columns of every step
 //   warps 16..19 store an item's gradients while the others go on with the next item
 //   warp 20      producer: finds items, loads their operands (two slots) and the stream (TMA ring)
-//   warp 23      splits lse and D of the streamed queries of key items (below)
+//   warp 23      splits lse and D of the streamed queries of key items (below), and clears the rows behind a
+//                sequence's end in its last tile
 //   warp 21      issues the scores' MMAs: those of step n + 3 once the products of step n have freed its buffer
 //   warp 22      issues the products' MMAs
 // Steps, buffers and stages are numbered through all items, so an item's first scores are computed while the
@@ -31,7 +32,7 @@
 // In key items lse and D belong to the columns of a thread's row. Reading them for every row costs more
 // shared-memory bandwidth than all operand reads of the tensor cores (a 16-byte broadcast read is four
 // wavefronts), so they are subtracted by the tensor cores: one more K step of 16 with the constants
-// (2^15, 1, 2^-14) in every row of A and -lse / scale, or -D, split into three parts of the operand type
+// (2^15, 1, 2^-10) in every row of A and -lse / scale, or -D, split into three parts of the operand type
 // in B, which represents fp32 values between about 2^-30 and 2^30 to 2^-24 or better.
 //
 // Heads narrower than 32 or 64 columns arrive zero-padded by the 3-D tensor maps. Rows past the
@@ -56,7 +57,7 @@ namespace {
 constexpr int kOwn = 128;      // rows an item owns
 constexpr int kStep = 64;      // rows of a streamed tile
 constexpr int kBufs = 3;       // score buffers
-constexpr int kElemWarps = 16, kTeams = 1, kTeamWarps = kElemWarps / kTeams;
+constexpr int kElemWarps = 16, kTeams = 2, kTeamWarps = kElemWarps / kTeams;
 constexpr int kWarpCols = 4 * kStep / kTeamWarps;  // columns of an elementwise warp
 constexpr int kStoreWarp = kElemWarps, kLoadWarp = kStoreWarp + 4;
 constexpr int kScoreWarp = kLoadWarp + 1, kProductWarp = kScoreWarp + 1, kSplitWarp = kProductWarp + 1;
@@ -162,46 +163,45 @@ __global__ void __launch_bounds__(256) attention_delta_kernel(const BwdParams p)
   }
 }
 
-// e: dS is rounded as 2^e dS. Called by a whole warp.
+// e: dS is rounded as 2^e dS.
 template <typename E>
-__device__ __forceinline__ int ds_exponent(const BwdParams& p, int start, int len, int b, int h, int lane) {
+__device__ __forceinline__ int ds_exponent(const BwdParams& p, int start, int len, int b, int h) {
   if constexpr (!std::is_same<E, __half>::value) return 0;
   const float* g = p.peaks + static_cast<size_t>(h) * p.blocks + row_block(start, b, 0);
   const float* v = g + static_cast<size_t>(p.H) * p.blocks;
   float top_g = 0.0f, top_v = 0.0f;
-  for (int i = lane; i < (len + kDeltaRows - 1) / kDeltaRows; i += 32) {
+#pragma unroll 8
+  for (int i = 0; i < (len + kDeltaRows - 1) / kDeltaRows; ++i) {
     top_g = fmaxf(top_g, g[i]);
     top_v = fmaxf(top_v, v[i]);
   }
-  const float bound = 2.0f * p.dh * warp_max(top_g) * warp_max(top_v);
+  const float bound = 2.0f * p.dh * top_g * top_v;
   if (!(bound > 0.0f)) return 0;
   return min(60, max(-60, 13 - ilogbf(bound)));
 }
 
-// x as three values of E, times 2^15, 1 and 2^-14 for fp16 (whose range the factors extend) and 1
+// x as three values of E, times 2^15, 1 and 2^-10 for fp16 (whose range the factors extend) and 1
 // for bf16, packed into the first 16 bytes of a K step (the other elements are zero).
 template <typename E>
 __device__ __forceinline__ uint4 split_parts(float x) {
-  float part[3];
   if constexpr (std::is_same<E, __half>::value) {
-    constexpr float kScale[3] = {32768.0f, 1.0f, 1.0f / 16384.0f};
-#pragma unroll
-    for (int i = 0; i < 3; ++i) {
-      part[i] = to_f32(from_f32<E>(fminf(fmaxf(x / kScale[i], -60000.0f), 60000.0f)));
-      x -= part[i] * kScale[i];
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 3; ++i) {
-      part[i] = to_f32(from_f32<E>(x));
-      x -= part[i];
-    }
+    const __half h0 = __float2half_rn(x * (1.0f / 32768.0f));
+    float r = fmaf(-32768.0f, __half2float(h0), x);
+    const __half h1 = __float2half_rn(fminf(fmaxf(r, -65504.0f), 65504.0f));
+    r = (r - __half2float(h1)) * 1024.0f;
+    const __half2 h01 = __halves2half2(h0, h1);
+    return make_uint4(*reinterpret_cast<const uint32_t*>(&h01), pack2<E>(r, 0.0f), 0u, 0u);
+  } else {  // by truncation: each part is the upper half of what is left
+    const uint32_t u0 = __float_as_uint(x);
+    float r = x - __uint_as_float(u0 & 0xffff0000u);
+    const uint32_t u1 = __float_as_uint(r);
+    r -= __uint_as_float(u1 & 0xffff0000u);
+    return make_uint4(__byte_perm(u0, u1, 0x7632), __float_as_uint(r) >> 16, 0u, 0u);
   }
-  return make_uint4(pack2<E>(part[0], part[1]), pack2<E>(part[2], 0.0f), 0u, 0u);
 }
 template <typename E>
 __device__ __forceinline__ uint4 split_factors() {
-  if constexpr (std::is_same<E, __half>::value) return make_uint4(pack2<E>(32768.0f, 1.0f), pack2<E>(1.0f / 16384.0f, 0.0f), 0u, 0u);
+  if constexpr (std::is_same<E, __half>::value) return make_uint4(pack2<E>(32768.0f, 1.0f), pack2<E>(1.0f / 1024.0f, 0.0f), 0u, 0u);
   else return make_uint4(pack2<E>(1.0f, 1.0f), pack2<E>(1.0f, 0.0f), 0u, 0u);
 }
 
@@ -220,7 +220,8 @@ __device__ __forceinline__ int swizzled(int row, int chunk) {
 template <int DH, typename E>
 __global__ void __launch_bounds__(kThreads, 1)
     attention_backward_kernel(const __grid_constant__ CUtensorMap tm_qkv, const __grid_constant__ CUtensorMap tm_dout,
-                              const BwdParams p) {
+                              const __grid_constant__ CUtensorMap tm_qkv_own,
+                              const __grid_constant__ CUtensorMap tm_dout_own, const BwdParams p) {
   using G = Bwd<DH>;
   constexpr int kStages = G::kStages;
   constexpr bool kScaled = std::is_same<E, __half>::value;
@@ -238,8 +239,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* probs = scores + kBufs;          // [kBufs] P and dS written
   uint64_t* done = probs + kBufs;            // an item's products finished
   uint64_t* acc_free = done + 1;             // its accumulators read
-  uint64_t* tail = acc_free + 1;             // a sequence's last tile has landed
-  uint64_t* drain = tail + 1;                // [2] everything an issuer issued
+  uint64_t* tail = acc_free + 1;             // [kStages] a sequence's last, partial tile has landed
+  uint64_t* drain = tail + kStages;                // [2] everything an issuer issued
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 2);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -252,6 +253,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&full[i], 2);  // the copies; the parts of lse and D, or for query items the producer again
       mbar_init(&empty[i], 1);
+      mbar_init(&tail[i], 1);
     }
     for (int i = 0; i < kBufs; ++i) {
       mbar_init(&scores[i], 1);
@@ -259,7 +261,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     mbar_init(done, 1);
     mbar_init(acc_free, 4);
-    mbar_init(tail, 1);
     for (int i = 0; i < 2; ++i) mbar_init(&drain[i], 1);
     fence_mbar_init();
   }
@@ -287,20 +288,19 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int tiles = (p.max_len + kOwn - 1) / kOwn;
     const int64_t half = static_cast<int64_t>(tiles) * p.H * p.B, total = 2 * half;
     bool ok = true;
-    int item = 0, n = 0, tails = 0;
+    int item = 0, n = 0;
     // Loads in flight when a wait gives up must land before the block exits.
     int own_loaded = 0;
     for (int64_t base = blockIdx.x; base < total && ok; base += static_cast<int64_t>(32) * gridDim.x) {
       // 32 candidates at a time, one per lane.
       const int64_t at = base + static_cast<int64_t>(lane) * gridDim.x;
       Item it{};
-      int b = 0;
       if (at < total) {
         const int64_t r = at < half ? at : at - half;
         it.keys = at < half;
         it.r0 = static_cast<int>(r % tiles) * kOwn;
         it.h = static_cast<int>(r / tiles % p.H);
-        b = static_cast<int>(r / tiles / p.H);
+        const int b = static_cast<int>(r / tiles / p.H);
         it.start = p.cu[b];
         it.len = p.cu[b + 1] - it.start;
         if (!packed_rows(it.start, it.len, p.T, p.max_len)) {
@@ -308,6 +308,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           it.len = 0;
         }
         if (it.r0 >= it.len) it.len = 0;
+        if (it.len > 0) it.ds_exp = ds_exponent<E>(p, it.start, it.len, b, it.h);
       }
       for (uint32_t found = __ballot_sync(0xffffffffu, it.len > 0); found != 0 && ok; found &= found - 1) {
         const int src = __ffs(found) - 1;
@@ -317,8 +318,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         cur.r0 = __shfl_sync(0xffffffffu, it.r0, src);
         cur.h = __shfl_sync(0xffffffffu, it.h, src);
         cur.keys = __shfl_sync(0xffffffffu, it.keys, src);
-        const int cb = __shfl_sync(0xffffffffu, b, src);
-        cur.ds_exp = ds_exponent<E>(p, cur.start, cur.len, cb, cur.h, lane);
+        cur.ds_exp = __shfl_sync(0xffffffffu, it.ds_exp, src);
         const int slot = item & 1, h = cur.h, len = cur.len, start = cur.start;
         const bool keys = cur.keys;
         ok = mbar_wait_spin(&own_empty[slot], ((item >> 1) & 1) ^ 1u, p.err, kDevTimeoutProducer);
@@ -326,53 +326,31 @@ __global__ void __launch_bounds__(kThreads, 1)
           ok = false;
           break;
         }
+        // Owned and streamed operands: head h1 of qkv, and head h2 of qkv or dO.
         if (lane == 0) {
           *info_at(item) = cur;
           mbar_arrive(&info_full[item % kInfos]);
           mbar_arrive_expect_tx(&own_full[slot], 2 * G::kOwnBytes);
           uint8_t* dst = smem + slot * 2 * G::kOwnBytes;
-          for (int i = 0; i < 2; ++i) {
-            const int row = start + cur.r0 + i * kStep;
-            tma_load_3d(dst + i * G::kTileBytes, &tm_qkv, &own_full[slot], 0, keys ? p.H + h : h, row, pol);
-            tma_load_3d(dst + G::kOwnBytes + i * G::kTileBytes, keys ? &tm_qkv : &tm_dout, &own_full[slot], 0,
-                        keys ? 2 * p.H + h : h, row, pol);
-          }
-        }
-        own_loaded = item + 1;
-        for (int j = 0; j * kStep < len; ++j, ++n) {
-          const int st = n % kStages, kept = len - j * kStep;  // rows of this tile inside the sequence
-          ok = mbar_wait_spin(&empty[st], ((n / kStages) & 1) ^ 1u, p.err, kDevTimeoutProducer);
-          if (!__all_sync(0xffffffffu, ok)) {
-            ok = false;
-            break;
-          }
-          uint8_t* dst = smem + G::kOffStream + st * G::kStageBytes;
-          if (lane == 0) {
-            uint64_t* bar = kept < kStep ? tail : &full[st];
+          tma_load_3d(dst, &tm_qkv_own, &own_full[slot], 0, keys ? p.H + h : h, start + cur.r0, pol);
+          tma_load_3d(dst + G::kOwnBytes, keys ? &tm_qkv_own : &tm_dout_own, &own_full[slot], 0, keys ? 2 * p.H + h : h,
+                      start + cur.r0, pol);
+          own_loaded = item + 1;
+          const int h1 = keys ? h : p.H + h, h2 = keys ? h : 2 * p.H + h;
+          const CUtensorMap* map2 = keys ? &tm_dout : &tm_qkv;
+          for (int row = 0; row < len; row += kStep) {
+            const int st = n % kStages;
+            if (!(ok = mbar_wait_spin(&empty[st], ((n / kStages) & 1) ^ 1u, p.err, kDevTimeoutProducer))) break;
+            uint8_t* to = smem + G::kOffStream + st * G::kStageBytes;
+            uint64_t* bar = len - row < kStep ? &tail[st] : &full[st];
             mbar_arrive_expect_tx(bar, 2 * G::kTileBytes);
-            const int row = start + j * kStep;
-            tma_load_3d(dst, &tm_qkv, bar, 0, keys ? h : p.H + h, row, pol);
-            tma_load_3d(dst + G::kTileBytes, keys ? &tm_dout : &tm_qkv, bar, 0, keys ? h : 2 * p.H + h, row, pol);
+            tma_load_3d(to, &tm_qkv, bar, 0, h1, start + row, pol);
+            tma_load_3d(to + G::kTileBytes, map2, bar, 0, h2, start + row, pol);
+            if (!keys) mbar_arrive(&full[st]);
+            ++n;
           }
-          if (kept < kStep) {
-            ok = mbar_wait_spin(tail, tails & 1, p.err, kDevTimeoutProducer);
-            if (!__all_sync(0xffffffffu, ok)) {
-              ok = false;
-              break;
-            }
-            ++tails;
-            // Rows stay whole under the swizzle.
-            constexpr int kRow = DH * 2 / 16;
-            for (int i = kept * kRow + lane; i < kStep * kRow; i += 32) {
-              reinterpret_cast<uint4*>(dst)[i] = make_uint4(0u, 0u, 0u, 0u);
-              reinterpret_cast<uint4*>(dst + G::kTileBytes)[i] = make_uint4(0u, 0u, 0u, 0u);
-            }
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&full[st]);
-          }
-          if (!keys && lane == 0) mbar_arrive(&full[st]);
         }
+        ok = __shfl_sync(0xffffffffu, ok, 0);
         ++item;
       }
     }
@@ -385,7 +363,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else if (lane == 0) {
       for (int i = own_loaded > 2 ? own_loaded - 2 : 0; i < own_loaded; ++i)
         mbar_wait(&own_full[i & 1], (i >> 1) & 1, p.err, kDevTimeoutProducer);
-      for (int i = n > kStages ? n - kStages : 0; i < n; ++i)
+      for (int i = n > kStages ? n - kStages : 0; i < n; ++i)  // a partial tile's through the clearing warp
         mbar_wait(&full[i % kStages], (i / kStages) & 1, p.err, kDevTimeoutProducer);
     }
   } else if (warp == kScoreWarp) {
@@ -492,7 +470,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ---------------- parts of lse and D of the streamed queries (key items) ----------------
     const float inv_scale = 1.0f / p.scale;
     bool ok = true;
-    int st = 0, phase = 1;  // the stage's turn, and the parity of its release before that
+    int st = 0, phase = 1;      // the stage's turn, and the parity of its release before that
+    uint32_t tail_phases = 0;   // bit per stage
     for (int item = 0; ok; ++item) {
       if (!mbar_wait_spin(&info_full[item % kInfos], (item / kInfos) & 1, p.err, kDevTimeoutProducer)) break;
       const Item it = *info_at(item);
@@ -510,27 +489,45 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       if (it.keys) stats(0);
       for (int j = 0; j * kStep < it.len; ++j) {
+        const int kept = it.len - j * kStep;  // rows of this tile inside the sequence
+        uint8_t* tile = smem + G::kOffStream + st * G::kStageBytes;
         if (it.keys) {
           uint4 part_l[2], part_d[2];
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
             // P = exp2(c (S - lse / scale)), times 2^kProbExp; 0 past the end.
-            const float x = j * kStep + lane + 32 * u < it.len ? -(next_l[u] - kProbExp * 0.69314718f) * inv_scale : (kScaled ? -1.9e9f : -1e30f);
+            const float x = lane + 32 * u < kept ? -(next_l[u] - kProbExp * 0.69314718f) * inv_scale : (kScaled ? -1.9e9f : -1e30f);
             part_l[u] = split_parts<E>(x);
             part_d[u] = split_parts<E>(-next_d[u]);
           }
           stats(j + 1);
           ok = __all_sync(0xffffffffu, mbar_wait_spin(&empty[st], phase, p.err, kDevTimeoutProducer));
           if (!ok) break;
-          uint8_t* parts = smem + G::kOffStream + st * G::kStageBytes + 2 * G::kTileBytes;
+          uint8_t* parts = tile + 2 * G::kTileBytes;
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
             *reinterpret_cast<uint4*>(parts + swizzled<DH>(lane + 32 * u, 0)) = part_l[u];
             *reinterpret_cast<uint4*>(parts + swizzled<DH>(lane + 32 * u, 2)) = part_d[u];
           }
+        }
+        if (kept < kStep) {
+          ok = __all_sync(0xffffffffu, mbar_wait_spin(&tail[st], (tail_phases >> st) & 1, p.err, kDevTimeoutProducer));
+          if (!ok) break;
+          tail_phases ^= 1u << st;
+          // Rows stay whole under the swizzle.
+          constexpr int kRow = DH * 2 / 16;
+          for (int i = kept * kRow + lane; i < kStep * kRow; i += 32) {
+            reinterpret_cast<uint4*>(tile)[i] = make_uint4(0u, 0u, 0u, 0u);
+            reinterpret_cast<uint4*>(tile + G::kTileBytes)[i] = make_uint4(0u, 0u, 0u, 0u);
+          }
+        }
+        if (it.keys || kept < kStep) {
           fence_proxy_async_smem();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&full[st]);
+          if (lane == 0) {
+            mbar_arrive(&full[st]);
+            if (it.keys && kept < kStep) mbar_arrive(&full[st]);
+          }
         }
         if (++st == kStages) {
           st = 0;
@@ -689,9 +686,11 @@ __global__ void __launch_bounds__(kThreads, 1)
 template <int DH, typename E>
 cudaError_t backward(const AttnOp& a, const BwdParams& p, cudaStream_t s) {
   constexpr bool kBf16 = std::is_same<E, __nv_bfloat16>::value;
-  CUtensorMap tm_qkv, tm_dout;
+  CUtensorMap tm_qkv, tm_dout, tm_qkv_own, tm_dout_own;  // boxes of 64 streamed and 128 owned rows
   if (!make_tmap_op_heads(&tm_qkv, a.qkv, kBf16, a.T, 3 * a.H, a.dh, a.ld_qkv, kStep) ||
-      !make_tmap_op_heads(&tm_dout, a.dout, kBf16, a.T, a.H, a.dh, a.ld_dout, kStep))
+      !make_tmap_op_heads(&tm_dout, a.dout, kBf16, a.T, a.H, a.dh, a.ld_dout, kStep) ||
+      !make_tmap_op_heads(&tm_qkv_own, a.qkv, kBf16, a.T, 3 * a.H, a.dh, a.ld_qkv, kOwn) ||
+      !make_tmap_op_heads(&tm_dout_own, a.dout, kBf16, a.T, a.H, a.dh, a.ld_dout, kOwn))
     return cudaErrorInvalidValue;
   static std::atomic<unsigned long long> configured{0};
   cudaError_t e = allow_smem(attention_backward_kernel<DH, E>, Bwd<DH>::kSmem, configured);
@@ -699,7 +698,8 @@ cudaError_t backward(const AttnOp& a, const BwdParams& p, cudaStream_t s) {
   attention_delta_kernel<E><<<dim3((a.max_len + kDeltaRows - 1) / kDeltaRows, a.H, a.B), 256, 0, s>>>(p);
   const int64_t items = static_cast<int64_t>(2) * ((a.max_len + kOwn - 1) / kOwn) * a.H * a.B;
   attention_backward_kernel<DH, E>
-      <<<static_cast<unsigned>(std::min<int64_t>(items, a.num_sms)), kThreads, Bwd<DH>::kSmem, s>>>(tm_qkv, tm_dout, p);
+      <<<static_cast<unsigned>(std::min<int64_t>(items, a.num_sms)), kThreads, Bwd<DH>::kSmem, s>>>(tm_qkv, tm_dout, tm_qkv_own,
+                                                                                                   tm_dout_own, p);
   return cudaGetLastError();
 }
 
