@@ -1833,21 +1833,21 @@ int check_buffers(esm_ctx* c, const Buffer* b, int n, cudaStream_t s) {
     if (dev != c->device) return fail(c, ESM_EINVAL, "the stream belongs to another device than the context");
   }
   for (int i = 0; i < n; ++i) {
-    const std::string name = b[i].name;
+    const char* name = b[i].name;  // a message is only built when there is one to give
     if (!b[i].p) {
       if (b[i].optional) continue;
-      return fail(c, ESM_EINVAL, name + " is null");
+      return fail(c, ESM_EINVAL, std::string(name) + " is null");
     }
-    if (b[i].ld < b[i].cols) return fail(c, ESM_EINVAL, name + ": the row stride is smaller than a row");
+    if (b[i].ld < b[i].cols) return fail(c, ESM_EINVAL, std::string(name) + ": the row stride is smaller than a row");
     if (b[i].begin() % b[i].align || (b[i].align > b[i].size && b[i].rows > 1 && b[i].ld * b[i].size % b[i].align))
-      return fail(c, ESM_EINVAL, name + ": rows must start on " + std::to_string(b[i].align) + "-byte boundaries");
+      return fail(c, ESM_EINVAL, std::string(name) + ": rows must start on " + std::to_string(b[i].align) + "-byte boundaries");
     cudaPointerAttributes a{};
     if (cudaPointerGetAttributes(&a, b[i].p) != cudaSuccess) {
       cudaGetLastError();
-      return fail(c, ESM_EINVAL, name + " is not device memory");
+      return fail(c, ESM_EINVAL, std::string(name) + " is not device memory");
     }
     if (a.type != cudaMemoryTypeManaged && (a.type != cudaMemoryTypeDevice || a.device != c->device))
-      return fail(c, ESM_EINVAL, name + " is not memory of the context's device");
+      return fail(c, ESM_EINVAL, std::string(name) + " is not memory of the context's device");
   }
   for (int i = 0; i < n; ++i)
     for (int j = i + 1; j < n; ++j)

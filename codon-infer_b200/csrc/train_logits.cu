@@ -7,10 +7,8 @@
 //     dx_j = dloss tau (q_j - sum of the p_i with id_i = j).
 //
 // Two forms of each, both bound by HBM at size and by latency below:
-//   V <= kSmallV (the encoder's 33 tokens): one row per thread. A warp copies its 32 rows, which are
-//     one contiguous piece of memory when ld = V, into shared memory at an odd pitch, so that reading
-//     along a row is free of bank conflicts, and every row's work is serial: no shuffles, and a gradient
-//     row is finished in shared memory before it is written.
+//   V <= kSmallV (the encoder's 33 tokens): four lanes per row, which keep its elements in registers, so a
+//     row is read once, reductions take two shuffles, and eight rows share a warp's instructions.
 //   larger V: one block per row and a running maximum and sum, so x is read once for the sums. The
 //     top k come from a second pass (out of L2) that collects what reaches a threshold at least k
 //     elements are known to reach: see row_top.
@@ -36,188 +34,199 @@ __device__ __forceinline__ float key_value(uint32_t u) {
   return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);
 }
 
-// ---- one row per thread --------------------------------------------------------------------------
+// ---- four lanes per row -----------------------------------------------------------------------------
 
-// Calls f(row, column) for the rows x cols elements of a warp's rows, in memory order.
-template <typename F>
-__device__ __forceinline__ void warp_elements(int rows, int cols, F f) {
-  const int lane = threadIdx.x & 31, q = 32 / cols, m = 32 % cols;
-  int r = lane / cols, c = lane % cols;
-#pragma unroll 4
-  for (int i = lane; i < rows * cols; i += 32) {
-    f(r, c);
-    r += q;
-    c += m;
-    if (c >= cols) {
-      c -= cols;
-      ++r;
-    }
-  }
+// Lane q of a row's four has elements q, q + 4, .. (N of them, -inf past the end).
+template <typename E, int N>
+__device__ __forceinline__ void load_quad(const E* x, int V, int q, float (&v)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = q + 4 * i < V ? to_f32(x[q + 4 * i]) : -INFINITY;
+}
+__device__ __forceinline__ float quad_sum(float v) {
+  v += __shfl_xor_sync(0xffffffffu, v, 1);
+  return v + __shfl_xor_sync(0xffffffffu, v, 2);
+}
+__device__ __forceinline__ float quad_max(float v) {
+  v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
+  return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
 }
 
-// The 32 rows of a warp and their shared memory: `x` (pitch V | 1), and two arrays of pitch k | 1.
-struct WarpRows {
-  int64_t r0;
-  int rows, lane, px, pk;
-  float *x, *a, *b;
-  __device__ WarpRows(const LogitsOp& p, float* smem) {
-    const int warp = threadIdx.x >> 5;
-    lane = threadIdx.x & 31;
-    px = p.V | 1;
-    pk = p.k | 1;
-    r0 = (static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + warp) * 32;
-    rows = static_cast<int>(min(static_cast<int64_t>(32), p.T - r0));
-    x = smem + static_cast<size_t>(warp) * 32 * (px + 2 * pk);
-    a = x + 32 * px;
-    b = a + 32 * pk;
+// A block of 128 threads has 32 rows; lanes past the last row work on it again and write nothing.
+struct QuadRow {
+  int64_t t;
+  int q;
+  bool real;
+  __device__ explicit QuadRow(int T) {
+    const int64_t r = static_cast<int64_t>(blockIdx.x) * 32 + (threadIdx.x >> 2);
+    real = r < T;
+    t = real ? r : T - 1;
+    q = threadIdx.x & 3;
   }
 };
-size_t warp_rows_bytes(const LogitsOp& p) { return 32 * sizeof(float) * ((p.V | 1) + 2 * (p.k | 1)); }
 
-template <typename E>
-__global__ void logprobs_small_kernel(const LogitsOp p) {
-  extern __shared__ float smem_f[];
-  const WarpRows w(p, smem_f);
-  if (w.rows <= 0) return;
-  const E* x = static_cast<const E*>(p.logits);
-  warp_elements(w.rows, p.V, [&](int r, int c) { w.x[r * w.px + c] = to_f32(x[(w.r0 + r) * p.ld + c]); });
-  __syncwarp();
-  if (w.lane < w.rows) {
-    const int64_t t = w.r0 + w.lane;
-    float* row = w.x + w.lane * w.px;
-    float m = -INFINITY;
-    for (int j = 0; j < p.V; ++j) m = fmaxf(m, row[j]);
-    float s = 0.0f, u = 0.0f;
-#pragma unroll 4
-    for (int j = 0; j < p.V; ++j) {
-      const float v = row[j] - m, e = fast_exp2(v * kLog2e);
+template <typename E, int N>
+__global__ void __launch_bounds__(128) logprobs_quad_kernel(const LogitsOp p) {
+  const QuadRow r(p.T);
+  const E* x = static_cast<const E*>(p.logits) + r.t * p.ld;
+  float v[N];
+  load_quad<E, N>(x, p.V, r.q, v);
+  const int target = p.targets ? p.targets[r.t] : -1;
+  float m = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < N; ++i) m = fmaxf(m, v[i]);
+  m = quad_max(m);
+  float s = 0.0f, u = 0.0f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if (r.q + 4 * i < p.V) {
+      const float d = v[i] - m, e = fast_exp2(d * kLog2e);
       s += e;
-      u += e > 0.0f ? e * v : 0.0f;  // a NaN reaches s
+      u += e > 0.0f ? e * d : 0.0f;  // a NaN reaches s
     }
-    const float log_s = logf(s);
-    if (p.entropy) p.entropy[t] = s == s ? log_s - u / s : s;
-    if (p.logp) {
-      const int id = p.targets[t];
-      p.logp[t] = id >= 0 && id < p.V ? row[id] - m - log_s : 0.0f;
-    }
-    if (p.k > 0) {
-      // k times the best key that is left; the first of equal ones.
-      uint32_t* keys = reinterpret_cast<uint32_t*>(row);
-      for (int j = 0; j < p.V; ++j) keys[j] = order_key(row[j]);
-      for (int i = 0; i < p.k; ++i) {
-        uint32_t best = 0;
-        int id = 0;
-#pragma unroll 4
-        for (int j = 0; j < p.V; ++j) {
-          const uint32_t key = keys[j];
-          if (key > best) {
-            best = key;
-            id = j;
-          }
-        }
-        keys[id] = 0;
-        w.a[w.lane * w.pk + i] = __int_as_float(s == s ? id : -1);
-        w.b[w.lane * w.pk + i] = s == s ? key_value(best) - m - log_s : s;
+  }
+  s = quad_sum(s);
+  u = quad_sum(u);
+  const bool none = s != s;
+  const float log_s = logf(s);
+  if (r.real && r.q == 0) {
+    if (p.entropy) p.entropy[r.t] = none ? NAN : log_s - u / s;
+    if (p.logp) p.logp[r.t] = target >= 0 && target < p.V ? to_f32(x[target]) - m - log_s : 0.0f;
+  }
+  if (p.k == 0) return;
+  // k times the best key that is left, the first of equal ones; taken and missing elements have key 0.
+  uint32_t key[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) key[i] = r.q + 4 * i < p.V ? order_key(v[i]) : 0u;
+  for (int i = 0; i < p.k; ++i) {
+    uint32_t best = 0;
+    int id = r.q;
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (key[j] > best) {
+        best = key[j];
+        id = r.q + 4 * j;
+      }
+#pragma unroll
+    for (int o = 1; o <= 2; o <<= 1) {
+      const uint32_t other = __shfl_xor_sync(0xffffffffu, best, o);
+      const int other_id = __shfl_xor_sync(0xffffffffu, id, o);
+      if (other > best || (other == best && other_id < id)) {
+        best = other;
+        id = other_id;
       }
     }
-  }
-  if (p.k > 0) {
-    __syncwarp();
-    warp_elements(w.rows, p.k, [&](int r, int c) {
-      p.top_ids[(w.r0 + r) * p.k + c] = __float_as_int(w.a[r * w.pk + c]);
-      p.top_logp[(w.r0 + r) * p.k + c] = w.b[r * w.pk + c];
-    });
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (r.q + 4 * j == id) key[j] = 0;
+    if (r.real && r.q == (i & 3)) {
+      p.top_ids[r.t * p.k + i] = none ? -1 : id;
+      p.top_logp[r.t * p.k + i] = none ? NAN : key_value(best) - m - log_s;
+    }
   }
 }
 
-// The teacher's part of a row: ids in `id` (as bits, -1 where absent), logits in `v`, which become the
-// probabilities. Returns whether there are any; *log_scale is what makes (v - top) / tau a log
-// probability.
-struct Teacher {
+// The teacher's alternatives of a row of four lanes: lane q has i = q, q + 4, ..; ids -1 where absent.
+constexpr int kQuadAlts = ESM_MAX_ALTERNATIVES / 4;
+template <int K>
+struct QuadTeacher {
+  int id[K];
+  float v[K];  // logits, then log probabilities
   bool any;
-  float top, log_s;
+  __device__ __forceinline__ void load(const LogitsOp& p, const QuadRow& r) {
+#pragma unroll
+    for (int c = 0; c < K; ++c) {
+      const int i = r.q + 4 * c;
+      id[c] = i < p.k ? p.alt_ids[r.t * p.k + i] : -1;
+      v[c] = i < p.k ? p.alt_logits[r.t * p.k + i] : -INFINITY;
+    }
+  }
+  __device__ __forceinline__ void normalise(int V, float inv_tau) {
+    float top = -INFINITY, s = 0.0f;
+#pragma unroll
+    for (int c = 0; c < K; ++c) {
+      if (id[c] < 0 || id[c] >= V) {
+        id[c] = -1;
+        v[c] = -INFINITY;
+      }
+      top = fmaxf(top, v[c]);
+    }
+    top = quad_max(top);
+    any = top > -INFINITY;
+#pragma unroll
+    for (int c = 0; c < K; ++c) {
+      v[c] = (v[c] - top) * inv_tau;
+      s += id[c] >= 0 ? fast_exp2(v[c] * kLog2e) : 0.0f;
+    }
+    const float log_s = logf(quad_sum(s));
+#pragma unroll
+    for (int c = 0; c < K; ++c) v[c] -= log_s;
+  }
+  __device__ __forceinline__ float prob(int c) const { return id[c] >= 0 ? fast_exp2(v[c] * kLog2e) : 0.0f; }
 };
-__device__ __forceinline__ Teacher teacher_row(float* id, float* v, int k, int V, float inv_tau) {
-  Teacher t{false, -INFINITY, 0.0f};
-  for (int i = 0; i < k; ++i) {
-    const int a = __float_as_int(id[i]);
-    if (a < 0 || a >= V) {
-      id[i] = __int_as_float(-1);
-      v[i] = -INFINITY;
-    }
-    t.top = fmaxf(t.top, v[i]);
-  }
-  t.any = t.top > -INFINITY;
-  float s = 0.0f;
-  for (int i = 0; i < k; ++i) s += __float_as_int(id[i]) >= 0 ? fast_exp2((v[i] - t.top) * inv_tau * kLog2e) : 0.0f;
-  t.log_s = logf(s);
-  return t;
-}
 
-// Copies the warp's alternatives into shared memory: ids to w.a, logits to w.b.
-__device__ __forceinline__ void load_alternatives(const LogitsOp& p, const WarpRows& w) {
-  warp_elements(w.rows, p.k, [&](int r, int c) {
-    w.a[r * w.pk + c] = __int_as_float(p.alt_ids[(w.r0 + r) * p.k + c]);
-    w.b[r * w.pk + c] = p.alt_logits[(w.r0 + r) * p.k + c];
-  });
-}
-
-template <typename E>
-__global__ void distill_loss_small_kernel(const LogitsOp p) {
-  extern __shared__ float smem_f[];
-  const WarpRows w(p, smem_f);
-  if (w.rows <= 0) return;
-  const E* x = static_cast<const E*>(p.logits);
-  warp_elements(w.rows, p.V, [&](int r, int c) { w.x[r * w.px + c] = to_f32(x[(w.r0 + r) * p.ld + c]); });
-  load_alternatives(p, w);
-  __syncwarp();
-  if (w.lane >= w.rows) return;
-  const int64_t t = w.r0 + w.lane;
+template <typename E, int N, int K>
+__global__ void __launch_bounds__(128) distill_loss_quad_kernel(const LogitsOp p) {
+  const QuadRow r(p.T);
+  const E* x = static_cast<const E*>(p.logits) + r.t * p.ld;
   const float inv_tau = 1.0f / p.temperature;
-  const float* row = w.x + w.lane * w.px;
-  float *id = w.a + w.lane * w.pk, *v = w.b + w.lane * w.pk;
+  QuadTeacher<K> tr;
+  tr.load(p, r);
+  float v[N];
+  load_quad<E, N>(x, p.V, r.q, v);
   float m = -INFINITY, s = 0.0f;
-  for (int j = 0; j < p.V; ++j) m = fmaxf(m, row[j]);
-#pragma unroll 4
-  for (int j = 0; j < p.V; ++j) s += fast_exp2((row[j] - m) * inv_tau * kLog2e);
-  const float log_s = logf(s);
-  const Teacher tr = teacher_row(id, v, p.k, p.V, inv_tau);
+#pragma unroll
+  for (int i = 0; i < N; ++i) m = fmaxf(m, v[i]);
+  m = quad_max(m);
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (r.q + 4 * i < p.V) s += fast_exp2((v[i] - m) * inv_tau * kLog2e);
+  const float log_s = logf(quad_sum(s));
+  tr.normalise(p.V, inv_tau);
   float loss = 0.0f;
-  for (int i = 0; i < p.k; ++i) {
-    const int a = __float_as_int(id[i]);
-    const float logp = (v[i] - tr.top) * inv_tau - tr.log_s, pr = a >= 0 ? fast_exp2(logp * kLog2e) : 0.0f;
-    if (!(pr <= 0.0f)) loss += pr * (logp - ((row[a] - m) * inv_tau - log_s));
+#pragma unroll
+  for (int c = 0; c < K; ++c) {
+    const float pr = tr.prob(c);
+    if (!(pr <= 0.0f)) loss += pr * (tr.v[c] - ((to_f32(x[tr.id[c]]) - m) * inv_tau - log_s));
   }
-  p.loss[t] = tr.any ? p.temperature * p.temperature * loss : 0.0f;
-  p.lse[t] = m * inv_tau + log_s;
+  loss = quad_sum(loss);
+  if (r.real && r.q == 0) {
+    p.loss[r.t] = tr.any ? p.temperature * p.temperature * loss : 0.0f;
+    p.lse[r.t] = m * inv_tau + log_s;
+  }
 }
 
-template <typename E>
-__global__ void distill_backward_small_kernel(const LogitsOp p) {
-  extern __shared__ float smem_f[];
-  const WarpRows w(p, smem_f);
-  if (w.rows <= 0) return;
-  const E* x = static_cast<const E*>(p.logits);
-  E* dx = static_cast<E*>(p.dlogits);
-  warp_elements(w.rows, p.V, [&](int r, int c) { w.x[r * w.px + c] = to_f32(x[(w.r0 + r) * p.ld + c]); });
-  load_alternatives(p, w);
-  __syncwarp();
-  if (w.lane < w.rows) {
-    const int64_t t = w.r0 + w.lane;
-    const float inv_tau = 1.0f / p.temperature, g = p.dloss[t] * p.temperature, lse = p.lse[t];
-    float* row = w.x + w.lane * w.px;
-    float *id = w.a + w.lane * w.pk, *v = w.b + w.lane * w.pk;
-    const Teacher tr = teacher_row(id, v, p.k, p.V, inv_tau);
-    const bool none = !tr.any || g == 0.0f;
-#pragma unroll 4
-    for (int j = 0; j < p.V; ++j) row[j] = none ? 0.0f : g * fast_exp2((row[j] * inv_tau - lse) * kLog2e);
-    for (int i = 0; i < p.k && !none; ++i) {
-      const int a = __float_as_int(id[i]);
-      if (a >= 0) row[a] -= g * fast_exp2(((v[i] - tr.top) * inv_tau - tr.log_s) * kLog2e);
+template <typename E, int N, int K>
+__global__ void __launch_bounds__(128) distill_backward_quad_kernel(const LogitsOp p) {
+  const QuadRow r(p.T);
+  const E* x = static_cast<const E*>(p.logits) + r.t * p.ld;
+  E* dx = static_cast<E*>(p.dlogits) + r.t * p.ld_grad;
+  const float inv_tau = 1.0f / p.temperature, g = p.dloss[r.t] * p.temperature, lse = p.lse[r.t];
+  QuadTeacher<K> tr;
+  tr.load(p, r);
+  float v[N];
+  load_quad<E, N>(x, p.V, r.q, v);
+  tr.normalise(p.V, inv_tau);
+  const bool none = !tr.any || g == 0.0f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = fast_exp2((v[i] * inv_tau - lse) * kLog2e);
+  // Every alternative to all four lanes; the one that has its column subtracts its probability.
+#pragma unroll
+  for (int c = 0; c < K; ++c) {
+    if (4 * c >= p.k) break;
+    const float pr = tr.prob(c);
+#pragma unroll
+    for (int o = 0; o < 4; ++o) {
+      const int id = __shfl_sync(0xffffffffu, tr.id[c], o, 4);
+      const float pi = __shfl_sync(0xffffffffu, pr, o, 4);
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (id == r.q + 4 * i) v[i] -= pi;
     }
   }
-  __syncwarp();
-  warp_elements(w.rows, p.V, [&](int r, int c) { dx[(w.r0 + r) * p.ld_grad + c] = from_f32<E>(w.x[r * w.px + c]); });
+  if (!r.real) return;
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (r.q + 4 * i < p.V) dx[r.q + 4 * i] = from_f32<E>(none ? 0.0f : g * v[i]);
 }
 
 // ---- one block per row -----------------------------------------------------------------------------
@@ -261,22 +270,29 @@ struct Online {
   float m = -INFINITY, s = 0.0f, u = 0.0f;
 };
 
-template <bool ENTROPY, int N>
-__device__ __forceinline__ void online_add(Online& o, const float (&v)[N], int n, float c, float inv_tau) {
+// TOP: *at is the index of the first element that equals o.m (j that of v[0]).
+template <bool TOP, bool ENTROPY, int N>
+__device__ __forceinline__ void online_add(Online& o, int* at, int j, const float (&v)[N], int n, float c, float inv_tau) {
   float top = v[0];
 #pragma unroll
   for (int i = 1; i < N; ++i)
     if (i < n) top = fmaxf(top, v[i]);
-  if (top > o.m) {
+  if (top > o.m) {  // seldom, after the first few elements
     const float d = (o.m - top) * inv_tau, a = fast_exp2(d * kLog2e);
     if (ENTROPY) o.u = a > 0.0f ? a * (o.u + d * o.s) : 0.0f;  // d may be infinite where a is 0
     o.s = a * o.s;  // a is 0 where there was nothing; a NaN stays
     o.m = top;
+    if (TOP) {
+#pragma unroll
+      for (int i = N - 1; i >= 0; --i)
+        if (i < n && v[i] == top) *at = j + i;
+    }
   }
   if (o.m == -INFINITY) {  // nothing but -inf, or a NaN, so far
 #pragma unroll
     for (int i = 0; i < N; ++i)
       if (i < n && v[i] != v[i]) o.s = v[i];
+    if (TOP && *at < 0) *at = j;
     return;
   }
 #pragma unroll
@@ -284,7 +300,7 @@ __device__ __forceinline__ void online_add(Online& o, const float (&v)[N], int n
     if (i < n) {
       const float d = v[i] - o.m, e = fast_exp2(d * c);
       o.s += e;
-      if (ENTROPY) o.u += e > 0.0f ? e * d * inv_tau : 0.0f;
+      if (ENTROPY) o.u = fmaf(e, fmaxf(d, -1e30f), o.u);  // 0 where e is
     }
 }
 
@@ -313,13 +329,17 @@ __device__ __forceinline__ Online block_join(Online o, float inv_tau) {
     __shared__ Online sm[NT / 32];
     if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = o;
     __syncthreads();
-    o = Online();
-    for (int i = 0; i < NT / 32; ++i) online_join(o, sm[i].m, sm[i].s, sm[i].u, inv_tau);
-  } else {  // the lanes joined in different orders
-    o.m = __shfl_sync(0xffffffffu, o.m, 0);
-    o.s = __shfl_sync(0xffffffffu, o.s, 0);
-    o.u = __shfl_sync(0xffffffffu, o.u, 0);
+    o = (threadIdx.x & 31) < NT / 32 ? sm[threadIdx.x & 31] : Online();
+    for (int k = NT / 64; k > 0; k >>= 1) {
+      const float m = __shfl_xor_sync(0xffffffffu, o.m, k), s = __shfl_xor_sync(0xffffffffu, o.s, k);
+      const float u = __shfl_xor_sync(0xffffffffu, o.u, k);
+      online_join(o, m, s, u, inv_tau);
+    }
   }
+  // The lanes joined in different orders: all take the first one's.
+  o.m = __shfl_sync(0xffffffffu, o.m, 0);
+  o.s = __shfl_sync(0xffffffffu, o.s, 0);
+  o.u = __shfl_sync(0xffffffffu, o.u, 0);
   return o;
 }
 
@@ -361,7 +381,7 @@ __device__ void row_top(const LogitsOp& p, const E* x, int64_t t, float best, in
   row_elements<NT>(x, p.V, [&](int j, const auto& v, int n) {
 #pragma unroll
     for (int i = 0; i < static_cast<int>(sizeof(v) / 4); ++i)
-      if (i < n && v[i] >= floor_value) {
+      if (i < n && v[i] >= floor_value) {  // seldom
         const uint64_t c = static_cast<uint64_t>(order_key(v[i])) << 32 | ~static_cast<uint32_t>(j + i);
         if (c >= least) {
           const int slot = atomicAdd(&count, 1);
@@ -409,27 +429,17 @@ template <int NT, typename E>
 __global__ void __launch_bounds__(NT) logprobs_row_kernel(const LogitsOp p) {
   const int64_t t = blockIdx.x;
   const E* x = static_cast<const E*>(p.logits) + t * p.ld;
+  const int target = p.targets ? p.targets[t] : -1;
   Online o;
-  float best = -INFINITY;
   int at = -1;
-  row_elements<NT>(x, p.V, [&](int j, const auto& v, int n) {
-    online_add<true>(o, v, n, kLog2e, 1.0f);
-#pragma unroll
-    for (int i = 0; i < static_cast<int>(sizeof(v) / 4); ++i)
-      if (i < n && (v[i] > best || at < 0)) {
-        best = v[i];
-        at = j + i;
-      }
-  });
+  row_elements<NT>(x, p.V, [&](int j, const auto& v, int n) { online_add<true, true>(o, &at, j, v, n, kLog2e, 1.0f); });
+  const float best = o.m;
   o = block_join<NT>(o, 1.0f);
   if (threadIdx.x == 0) {
     const bool none = !(o.s == o.s) || o.m == -INFINITY;
     const float log_s = logf(o.s);
     if (p.entropy) p.entropy[t] = none ? NAN : log_s - o.u / o.s;
-    if (p.logp) {
-      const int id = p.targets[t];
-      p.logp[t] = id >= 0 && id < p.V ? (none ? NAN : to_f32(x[id]) - o.m - log_s) : 0.0f;
-    }
+    if (p.logp) p.logp[t] = target >= 0 && target < p.V ? (none ? NAN : to_f32(x[target]) - o.m - log_s) : 0.0f;
   }
   if (p.k > 0) row_top<NT>(p, x, t, best, at, o);
 }
@@ -466,17 +476,22 @@ __global__ void __launch_bounds__(NT) distill_loss_row_kernel(const LogitsOp p) 
   const int64_t t = blockIdx.x;
   const E* x = static_cast<const E*>(p.logits) + t * p.ld;
   const float inv_tau = 1.0f / p.temperature;
+  int id[2] = {-1, -1};
+  float pr[2], logp[2], at[2], loss = 0.0f;
+  bool any = false;
+  if (threadIdx.x < 32) {  // first, so that its loads' latency is not added to the row's
+    any = teacher(p, t, threadIdx.x, id, pr, logp);
+#pragma unroll
+    for (int c = 0; c < 2; ++c) at[c] = id[c] >= 0 ? to_f32(x[id[c]]) : 0.0f;
+  }
   Online o;
-  row_elements<NT>(x, p.V, [&](int, const auto& v, int n) { online_add<false>(o, v, n, inv_tau * kLog2e, inv_tau); });
+  row_elements<NT>(x, p.V, [&](int, const auto& v, int n) { online_add<false, false>(o, nullptr, 0, v, n, inv_tau * kLog2e, inv_tau); });
   o = block_join<NT>(o, inv_tau);
   if (threadIdx.x >= 32) return;
   const float log_s = logf(o.m == -INFINITY ? NAN : o.s);
-  int id[2];
-  float pr[2], logp[2], loss = 0.0f;
-  const bool any = teacher(p, t, threadIdx.x, id, pr, logp);
 #pragma unroll
   for (int c = 0; c < 2; ++c)
-    if (!(pr[c] <= 0.0f)) loss += pr[c] * (logp[c] - ((to_f32(x[id[c]]) - o.m) * inv_tau - log_s));
+    if (!(pr[c] <= 0.0f)) loss += pr[c] * (logp[c] - ((at[c] - o.m) * inv_tau - log_s));
   loss = warp_sum(loss);
   if (threadIdx.x == 0) {
     p.loss[t] = any ? p.temperature * p.temperature * loss : 0.0f;
@@ -537,62 +552,61 @@ __global__ void __launch_bounds__(NT) distill_backward_row_kernel(const LogitsOp
 
 // ---- launches ------------------------------------------------------------------------------------
 
-// Small rows: four warps a block once that fills the GPU, else one.
-struct SmallGrid {
-  unsigned blocks, threads;
-  size_t smem;
-  explicit SmallGrid(const LogitsOp& p) {
-    const unsigned warps = (static_cast<unsigned>(p.T) + 31) / 32;
-    // Up to 48 KB of shared memory a block; more than 24 KB a warp does not occur (V, k <= 64).
-    const unsigned per = warps >= 1024 && 4 * warp_rows_bytes(p) <= 48u << 10 ? 4 : 1;
-    blocks = (warps + per - 1) / per;
-    threads = 32 * per;
-    smem = per * warp_rows_bytes(p);
-  }
-};
+unsigned quads(const LogitsOp& p) { return (static_cast<unsigned>(p.T) + 31) / 32; }
+
+// Threads of a row's block: one warp for short rows; for long ones 512, or 256 where there are rows enough to
+// fill the GPU's 148 x 2048 threads with those, which then all run at once.
+int row_block(const LogitsOp& p) {
+  if (p.V <= 1024) return 32;
+  if (p.V <= 4096) return 128;
+  return p.T > 296 ? 256 : 512;
+}
 
 template <typename E>
 cudaError_t logprobs(const LogitsOp& p, cudaStream_t s) {
-  if (p.V <= kSmallV) {
-    const SmallGrid g(p);
-    logprobs_small_kernel<E><<<g.blocks, g.threads, g.smem, s>>>(p);
-  } else if (p.V <= 1024 && p.k <= 16) {  // a warp's 32 maxima bound the top k
-    logprobs_row_kernel<32, E><<<p.T, 32, 0, s>>>(p);
-  } else if (p.V <= 4096) {
-    logprobs_row_kernel<128, E><<<p.T, 128, 0, s>>>(p);
-  } else {
-    logprobs_row_kernel<512, E><<<p.T, 512, 0, s>>>(p);
-  }
+  const int nt = row_block(p);
+  if (p.V <= 40) logprobs_quad_kernel<E, 10><<<quads(p), 128, 0, s>>>(p);
+  else if (p.V <= kSmallV) logprobs_quad_kernel<E, 16><<<quads(p), 128, 0, s>>>(p);
+  else if (nt == 32 && p.k <= 16) logprobs_row_kernel<32, E><<<p.T, 32, 0, s>>>(p);  // a warp's 32 maxima bound the top k
+  else if (nt <= 128) logprobs_row_kernel<128, E><<<p.T, 128, 0, s>>>(p);
+  else if (nt == 256) logprobs_row_kernel<256, E><<<p.T, 256, 0, s>>>(p);
+  else logprobs_row_kernel<512, E><<<p.T, 512, 0, s>>>(p);
   return cudaGetLastError();
+}
+
+template <typename E, int N>
+void loss_quad(const LogitsOp& p, cudaStream_t s) {
+  if (p.k <= 16) distill_loss_quad_kernel<E, N, 4><<<quads(p), 128, 0, s>>>(p);
+  else distill_loss_quad_kernel<E, N, kQuadAlts><<<quads(p), 128, 0, s>>>(p);
 }
 
 template <typename E>
 cudaError_t loss(const LogitsOp& p, cudaStream_t s) {
-  if (p.V <= kSmallV) {
-    const SmallGrid g(p);
-    distill_loss_small_kernel<E><<<g.blocks, g.threads, g.smem, s>>>(p);
-  } else if (p.V <= 1024) {
-    distill_loss_row_kernel<32, E><<<p.T, 32, 0, s>>>(p);
-  } else if (p.V <= 4096) {
-    distill_loss_row_kernel<128, E><<<p.T, 128, 0, s>>>(p);
-  } else {
-    distill_loss_row_kernel<512, E><<<p.T, 512, 0, s>>>(p);
-  }
+  const int nt = row_block(p);
+  if (p.V <= 40) loss_quad<E, 10>(p, s);
+  else if (p.V <= kSmallV) loss_quad<E, 16>(p, s);
+  else if (nt == 32) distill_loss_row_kernel<32, E><<<p.T, 32, 0, s>>>(p);
+  else if (nt == 128) distill_loss_row_kernel<128, E><<<p.T, 128, 0, s>>>(p);
+  else if (nt == 256) distill_loss_row_kernel<256, E><<<p.T, 256, 0, s>>>(p);
+  else distill_loss_row_kernel<512, E><<<p.T, 512, 0, s>>>(p);
   return cudaGetLastError();
+}
+
+template <typename E, int N>
+void gradient_quad(const LogitsOp& p, cudaStream_t s) {
+  if (p.k <= 16) distill_backward_quad_kernel<E, N, 4><<<quads(p), 128, 0, s>>>(p);
+  else distill_backward_quad_kernel<E, N, kQuadAlts><<<quads(p), 128, 0, s>>>(p);
 }
 
 template <typename E>
 cudaError_t gradient(const LogitsOp& p, cudaStream_t s) {
-  if (p.V <= kSmallV) {
-    const SmallGrid g(p);
-    distill_backward_small_kernel<E><<<g.blocks, g.threads, g.smem, s>>>(p);
-  } else if (p.V <= 1024) {
-    distill_backward_row_kernel<32, E><<<p.T, 32, 0, s>>>(p);
-  } else if (p.V <= 4096) {
-    distill_backward_row_kernel<128, E><<<p.T, 128, 0, s>>>(p);
-  } else {
-    distill_backward_row_kernel<512, E><<<p.T, 512, 0, s>>>(p);
-  }
+  const int nt = row_block(p);
+  if (p.V <= 40) gradient_quad<E, 10>(p, s);
+  else if (p.V <= kSmallV) gradient_quad<E, 16>(p, s);
+  else if (nt == 32) distill_backward_row_kernel<32, E><<<p.T, 32, 0, s>>>(p);
+  else if (nt == 128) distill_backward_row_kernel<128, E><<<p.T, 128, 0, s>>>(p);
+  else if (nt == 256) distill_backward_row_kernel<256, E><<<p.T, 256, 0, s>>>(p);
+  else distill_backward_row_kernel<512, E><<<p.T, 512, 0, s>>>(p);
   return cudaGetLastError();
 }
 

@@ -180,37 +180,38 @@ _type_of: dict = {}  # dtype object -> element type
 
 
 def _element_type(t) -> int:
-    ty = _type_of.get(t.dtype)
-    if ty is None:
+    try:
+        return _type_of[t.dtype]
+    except KeyError:
         name = str(t.dtype).rsplit(".", 1)[-1]
         if name not in _ELEMENT_TYPES:
-            raise EsmError(ESM_EINVAL, f"element type {t.dtype} is not supported")
+            raise EsmError(ESM_EINVAL, f"element type {t.dtype} is not supported") from None
         ty = _type_of[t.dtype] = _ELEMENT_TYPES[name]
-    return ty
+        return ty
 
 
 def _bad(what: str):
     raise EsmError(ESM_EINVAL, what)
 
 
-def _rows(t, name: str, shape: tuple, types=None) -> tuple[int, int, int]:
+def _rows(t, name: str, shape: tuple, ty: int | None = None) -> tuple[int, int, int]:
     """(pointer, row stride, element type) of a CUDA matrix of `shape` whose rows are contiguous."""
-    if tuple(t.shape) != shape:
+    if t.shape != shape:
         _bad(f"{name} must have the shape {shape}, not {tuple(t.shape)}")
-    ty = _element_type(t)
-    if types is not None and ty not in types:
+    got = _element_type(t)
+    if ty is not None and got != ty:
         _bad(f"{name} has the element type {t.dtype}")
     ld, inner = t.stride()
-    if shape[1] > 1 and inner != 1:
+    if inner != 1 and shape[1] > 1:
         _bad(f"{name}: rows must be contiguous")
-    return t.data_ptr(), (ld if shape[0] > 1 else shape[1]), ty
+    return t.data_ptr(), (ld if shape[0] > 1 else shape[1]), got
 
 
 def _flat(t, name: str, shape: tuple, ty: int = TYPE_F32):
     """Pointer of a contiguous CUDA tensor of `shape` and element type `ty` (None stays None)."""
     if t is None:
         return None
-    if tuple(t.shape) != shape:
+    if t.shape != shape:
         _bad(f"{name} must have the shape {shape}, not {tuple(t.shape)}")
     if _element_type(t) != ty:
         _bad(f"{name} has the element type {t.dtype}")
@@ -537,7 +538,7 @@ class Model:
         T, d = out.shape
         dh = self._head_dim(d, n_heads)
         q, ldq, ty = _rows(qkv, "qkv", (T, 3 * d))
-        o, ldo, _ = _rows(out, "out", (T, d), (ty,))
+        o, ldo, _ = _rows(out, "out", (T, d), ty)
         B = cu_seqlens.shape[0] - 1
         rc = lib().esm_attention(self._ctx, ty, q, ldq, _flat(cu_seqlens, "cu_seqlens", (B + 1,), -1), B, T, max_len,
                                  n_heads, dh, dh ** -0.5 if scale is None else scale, o, ldo,
@@ -564,14 +565,14 @@ class Model:
         T, d = out.shape
         dh = self._head_dim(d, n_heads)
         q, ldq, ty = _rows(qkv, "qkv", (T, 3 * d))
-        o, ldo, _ = _rows(out, "out", (T, d), (ty,))
-        g, ldg, _ = _rows(dout, "dout", (T, d), (ty,))
-        dq, lddq, _ = _rows(dqkv, "dqkv", (T, 3 * d), (ty,))
+        o, ldo, _ = _rows(out, "out", (T, d), ty)
+        g, ldg, _ = _rows(dout, "dout", (T, d), ty)
+        dq, lddq, _ = _rows(dqkv, "dqkv", (T, 3 * d), ty)
         B = cu_seqlens.shape[0] - 1
         rc = lib().esm_attention_backward(self._ctx, ty, q, ldq, _flat(cu_seqlens, "cu_seqlens", (B + 1,), -1), B, T,
                                           max_len, n_heads, dh, dh ** -0.5 if scale is None else scale, o, ldo,
                                           _flat(lse, "lse", (n_heads, T)), g, ldg, dq, lddq, workspace.data_ptr(),
-                                          workspace.numel() * workspace.element_size(), _stream(stream))
+                                          workspace.nbytes, _stream(stream))
         self._chk(rc, "esm_attention_backward")
 
     def layernorm(self, x, w, b, y, mean=None, rstd=None, eps: float = 1e-5, stream=None) -> None:
@@ -598,7 +599,7 @@ class Model:
                                           _flat(w, "w", (d,)), _flat(mean, "mean", (T,)), _flat(rstd, "rstd", (T,)),
                                           _flat(dres, "dres", (T, d), xt), T, d, _flat(dx, "dx", (T, d), xt),
                                           _flat(dw, "dw", (d,)), _flat(db, "db", (d,)), workspace.data_ptr(),
-                                          workspace.numel() * workspace.element_size(), _stream(stream))
+                                          workspace.nbytes, _stream(stream))
         self._chk(rc, "esm_layernorm_backward")
 
     def token_logprobs(self, logits, targets=None, logp=None, entropy=None, top_ids=None, top_logp=None,
@@ -632,7 +633,7 @@ class Model:
         """dlogits [T, V], the gradient of sum_t dloss[t] * loss[t]; lse as distill_loss wrote it."""
         T, V = logits.shape
         x, ld, ty = _rows(logits, "logits", (T, V))
-        dx, ldg, _ = _rows(dlogits, "dlogits", (T, V), (ty,))
+        dx, ldg, _ = _rows(dlogits, "dlogits", (T, V), ty)
         k = top_ids.shape[1]
         rc = lib().esm_distill_backward(self._ctx, ty, x, ld, T, V, _flat(top_ids, "top_ids", (T, k), -1),
                                         _flat(top_logits, "top_logits", (T, k)), k, temperature,
