@@ -3,11 +3,13 @@
 //   g = dy w,  xh = (x - mean) rstd,  dx = rstd (g - mean(g) - xh mean(g xh)) + dres
 //   dw = sum over rows of dy xh,  db = sum over rows of dy
 // Bound by HBM. A block has one row in registers, NV vectors of VEC elements a thread, so x (and dy)
-// are read once. In the backward pass blocks stay: each takes every gridDim.x-th row, a thread adds
-// up dw and db of its own columns in registers over all of them, and the next row is loaded before
-// the current one's sums are exchanged. The blocks' sums go to the workspace and are added there in
-// order by layernorm_reduce_kernel, so the gradients do not depend on timing. Rows too wide for the
-// registers of a block (kMaxThreads * NV * VEC) take the looping kernels, which read them repeatedly.
+// are read once. Blocks stay and take every gridDim.x-th row. In the backward pass a block loads its next row
+// before the current one's sums are exchanged, and a thread adds up dw and db of its own columns in
+// registers over all its rows; the blocks' sums go to the workspace and are added there in order by
+// layernorm_reduce_kernel, so the gradients do not depend on timing. Small inputs, which stay in L2, take
+// one launch instead: some blocks compute dx, others read the same rows again for the columns of dw and db.
+// Rows too wide for the registers of a block (kMaxThreads * NV * VEC) take the looping kernels, which read
+// them repeatedly.
 #include <algorithm>
 
 #include "train_common.cuh"
@@ -38,55 +40,102 @@ __device__ __forceinline__ void block_sum2(float& a, float& b, float2* sm) {
   }
 }
 
+// The sum of v over the block.
+__device__ __forceinline__ float block_sum(float v, float* sm) {
+  v = warp_sum(v);
+  if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = 0.0f;
+  for (int i = 0; i < static_cast<int>(blockDim.x >> 5); ++i) v += sm[i];
+  return v;
+}
+
+// 65536 x 1280, fp32 to fp16: 88.6 us, 5.7 TB/s. The weights come from L1 for every row: in registers
+// they cost more blocks per SM than they save (103 us with them and the next row held there; 94 us with
+// a block per row).
 template <typename X, typename Y, int VEC, int NV>
 __global__ void __launch_bounds__(kMaxThreads) layernorm_row_kernel(const LayerNormOp p) {
-  __shared__ float2 sm[2][kMaxThreads / 32];
-  const size_t row = blockIdx.x;
-  const int n = p.d / VEC;
-  const Vec<X, VEC>* x = reinterpret_cast<const Vec<X, VEC>*>(static_cast<const X*>(p.x) + row * p.d);
-  const Vec<float, VEC>* w = reinterpret_cast<const Vec<float, VEC>*>(p.w);
-  const Vec<float, VEC>* b = reinterpret_cast<const Vec<float, VEC>*>(p.b);
-  Vec<X, VEC> raw[NV];
+  __shared__ float sm[2][2][kMaxThreads / 32];
+  const int n = p.d / VEC, t = threadIdx.x;
+  const float inv_d = 1.0f / p.d;
+  int turn = 0;
+  for (int64_t row = blockIdx.x; row < p.T; row += gridDim.x, turn ^= 1) {
+    const Vec<X, VEC>* x = reinterpret_cast<const Vec<X, VEC>*>(static_cast<const X*>(p.x) + row * p.d);
+    Vec<X, VEC> cur[NV];
 #pragma unroll
-  for (int k = 0; k < NV; ++k)
-    if (threadIdx.x + k * blockDim.x < n) raw[k] = x[threadIdx.x + k * blockDim.x];
-  float s = 0.0f, s2 = 0.0f;
+    for (int k = 0; k < NV; ++k)
+      if (t + k * static_cast<int>(blockDim.x) < n) cur[k] = x[t + k * blockDim.x];
+    float s = 0.0f;
 #pragma unroll
-  for (int k = 0; k < NV; ++k)
-    if (threadIdx.x + k * blockDim.x < n)
+    for (int k = 0; k < NV; ++k)
+      if (t + k * static_cast<int>(blockDim.x) < n)
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) s += to_f32(raw[k].v[i]);
-  block_sum2(s, s2, sm[0]);
-  const float mean = s / p.d;
-  s = s2 = 0.0f;
+        for (int i = 0; i < VEC; ++i) s += to_f32(cur[k].v[i]);
+    const float mean = block_sum(s, sm[turn][0]) * inv_d;
+    s = 0.0f;
 #pragma unroll
-  for (int k = 0; k < NV; ++k)
-    if (threadIdx.x + k * blockDim.x < n)
+    for (int k = 0; k < NV; ++k)
+      if (t + k * static_cast<int>(blockDim.x) < n)
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        const float v = to_f32(raw[k].v[i]) - mean;
-        s = fmaf(v, v, s);
+        for (int i = 0; i < VEC; ++i) {
+          const float v = to_f32(cur[k].v[i]) - mean;
+          s = fmaf(v, v, s);
+        }
+    const float rstd = 1.0f / sqrtf(block_sum(s, sm[turn][1]) * inv_d + p.eps);
+    Vec<Y, VEC>* y = reinterpret_cast<Vec<Y, VEC>*>(static_cast<Y*>(p.y) + row * p.d);
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+      if (t + k * static_cast<int>(blockDim.x) < n) {
+        const Vec<float, VEC> w = reinterpret_cast<const Vec<float, VEC>*>(p.w)[t + k * blockDim.x];
+        const Vec<float, VEC> b = reinterpret_cast<const Vec<float, VEC>*>(p.b)[t + k * blockDim.x];
+        Vec<Y, VEC> o;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) o.v[i] = from_f32<Y>(fmaf((to_f32(cur[k].v[i]) - mean) * rstd, w.v[i], b.v[i]));
+        y[t + k * blockDim.x] = o;
       }
-  block_sum2(s, s2, sm[1]);
-  const float rstd = 1.0f / sqrtf(s / p.d + p.eps);
-  Vec<Y, VEC>* y = reinterpret_cast<Vec<Y, VEC>*>(static_cast<Y*>(p.y) + row * p.d);
-#pragma unroll
-  for (int k = 0; k < NV; ++k)
-    if (threadIdx.x + k * blockDim.x < n) {
-      const Vec<float, VEC> wk = w[threadIdx.x + k * blockDim.x], bk = b[threadIdx.x + k * blockDim.x];
-      Vec<Y, VEC> o;
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) o.v[i] = from_f32<Y>(fmaf((to_f32(raw[k].v[i]) - mean) * rstd, wk.v[i], bk.v[i]));
-      y[threadIdx.x + k * blockDim.x] = o;
+    if (t == 0) {
+      if (p.mean) p.mean[row] = mean;
+      if (p.rstd) p.rstd[row] = rstd;
     }
-  if (threadIdx.x == 0) {
-    if (p.mean) p.mean[row] = mean;
-    if (p.rstd) p.rstd[row] = rstd;
   }
 }
 
-template <typename X, typename Y, int VEC, int NV, bool RES>
-__global__ void __launch_bounds__(kMaxThreads) layernorm_backward_kernel(const LayerNormOp p) {
+// SMALL: blocks [0, dx_blocks) of the launch compute dx alone, the others 32 columns of dw and db each.
+constexpr int kGroups = kMaxThreads / 32;
+template <typename X, typename Y>
+__device__ void layernorm_columns(const LayerNormOp& p, int block) {
+  __shared__ float sw[kGroups][33], sb[kGroups][33];
+  const int lane = threadIdx.x & 31, group = threadIdx.x >> 5, groups = blockDim.x >> 5, c = block * 32 + lane;
+  float dw = 0.0f, db = 0.0f;
+  if (c < p.d) {
+#pragma unroll 4
+    for (int r = group; r < p.T; r += groups) {
+      const size_t at = static_cast<size_t>(r) * p.d + c;
+      const float dy = to_f32(static_cast<const Y*>(p.dy)[at]);
+      dw = fmaf(dy, (to_f32(static_cast<const X*>(p.x)[at]) - p.mean[r]) * p.rstd[r], dw);
+      db += dy;
+    }
+  }
+  sw[group][lane] = dw;
+  sb[group][lane] = db;
+  __syncthreads();
+  if (group == 0 && c < p.d) {
+    dw = db = 0.0f;
+    for (int g = 0; g < groups; ++g) {
+      dw += sw[g][lane];
+      db += sb[g][lane];
+    }
+    p.dw[c] = dw;
+    p.db[c] = db;
+  }
+}
+
+template <typename X, typename Y, int VEC, int NV, bool RES, bool SMALL>
+__global__ void __launch_bounds__(kMaxThreads) layernorm_backward_kernel(const LayerNormOp p, const int dx_blocks) {
+  if (SMALL && static_cast<int>(blockIdx.x) >= dx_blocks) {
+    layernorm_columns<X, Y>(p, blockIdx.x - dx_blocks);
+    return;
+  }
   __shared__ float2 sm[2][kMaxThreads / 32];
   const int n = p.d / VEC, t = threadIdx.x;
   struct Row {
@@ -120,8 +169,8 @@ __global__ void __launch_bounds__(kMaxThreads) layernorm_backward_kernel(const L
   Row cur, next;
   int turn = 0;
   if (static_cast<int>(blockIdx.x) < p.T) load(cur, blockIdx.x);
-  for (int64_t row = blockIdx.x; row < p.T; row += gridDim.x, turn ^= 1) {
-    if (row + gridDim.x < p.T) load(next, row + gridDim.x);
+  for (int64_t row = blockIdx.x; row < p.T; row += dx_blocks, turn ^= 1) {
+    if (row + dx_blocks < p.T) load(next, row + dx_blocks);
     float a = 0.0f, b = 0.0f;
 #pragma unroll
     for (int k = 0; k < NV; ++k)
@@ -131,8 +180,10 @@ __global__ void __launch_bounds__(kMaxThreads) layernorm_backward_kernel(const L
           const float dy = to_f32(cur.dy[k].v[i]), xh = (to_f32(cur.x[k].v[i]) - cur.mean) * cur.rstd, g = dy * w[k].v[i];
           a += g;
           b = fmaf(g, xh, b);
-          dw[k].v[i] = fmaf(dy, xh, dw[k].v[i]);
-          db[k].v[i] += dy;
+          if constexpr (!SMALL) {
+            dw[k].v[i] = fmaf(dy, xh, dw[k].v[i]);
+            db[k].v[i] += dy;
+          }
         }
     block_sum2(a, b, sm[turn]);
     a *= inv_d;
@@ -153,6 +204,7 @@ __global__ void __launch_bounds__(kMaxThreads) layernorm_backward_kernel(const L
       }
     cur = next;
   }
+  if constexpr (SMALL) return;
   float* part = p.workspace + static_cast<size_t>(blockIdx.x) * 2 * p.d;
 #pragma unroll
   for (int k = 0; k < NV; ++k)
@@ -168,20 +220,18 @@ __global__ void __launch_bounds__(kMaxThreads) layernorm_backward_kernel(const L
 
 template <typename X, typename Y>
 __global__ void __launch_bounds__(kMaxThreads) layernorm_wide_kernel(const LayerNormOp p) {
-  __shared__ float2 sm[2][kMaxThreads / 32];
+  __shared__ float sm[2][kMaxThreads / 32];
   const size_t row = blockIdx.x;
   const X* x = static_cast<const X*>(p.x) + row * p.d;
-  float s = 0.0f, s2 = 0.0f;
+  float s = 0.0f;
   for (int c = threadIdx.x; c < p.d; c += kMaxThreads) s += to_f32(x[c]);
-  block_sum2(s, s2, sm[0]);
-  const float mean = s / p.d;
-  s = s2 = 0.0f;
+  const float mean = block_sum(s, sm[0]) / p.d;
+  s = 0.0f;
   for (int c = threadIdx.x; c < p.d; c += kMaxThreads) {
     const float v = to_f32(x[c]) - mean;
     s = fmaf(v, v, s);
   }
-  block_sum2(s, s2, sm[1]);
-  const float rstd = 1.0f / sqrtf(s / p.d + p.eps);
+  const float rstd = 1.0f / sqrtf(block_sum(s, sm[1]) / p.d + p.eps);
   Y* y = static_cast<Y*>(p.y) + row * p.d;
   for (int c = threadIdx.x; c < p.d; c += kMaxThreads)
     y[c] = from_f32<Y>(fmaf((to_f32(x[c]) - mean) * rstd, p.w[c], p.b[c]));
@@ -228,18 +278,20 @@ __global__ void __launch_bounds__(kMaxThreads) layernorm_wide_dw_kernel(const La
   p.workspace[static_cast<size_t>(blockIdx.y) * 2 * p.d + p.d + c] = db;
 }
 
-// ---- sums of the blocks' parts: 32 columns a block, 32 threads a column ---------------------------
+// ---- sums of the blocks' parts: 16 columns a block, 32 threads a column ---------------------------
 
-__global__ void __launch_bounds__(1024) layernorm_reduce_kernel(const float* part, int n, int d, float* dw, float* db) {
-  __shared__ float sm[32][33];
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
+__global__ void __launch_bounds__(512) layernorm_reduce_kernel(const float* part, int n, int d, float* dw, float* db) {
+  __shared__ float sm[32][17];
+  const int col = threadIdx.x & 15, w = threadIdx.x >> 4, c = blockIdx.x * 16 + col;
   float s = 0.0f;
-  if (c < 2 * d)
+  if (c < 2 * d) {
+#pragma unroll 8
     for (int i = w; i < n; i += 32) s += part[static_cast<size_t>(i) * 2 * d + c];
-  sm[w][lane] = s;
+  }
+  sm[w][col] = s;
   __syncthreads();
-  s = warp_sum(sm[lane][w]);
-  const int out = blockIdx.x * 32 + w;
+  const int lane = threadIdx.x & 31, column = threadIdx.x >> 5, out = blockIdx.x * 16 + column;
+  s = warp_sum(sm[lane][column]);
   if (lane == 0 && out < 2 * d) (out < d ? dw[out] : db[out - d]) = s;
 }
 
@@ -258,53 +310,67 @@ int row_threads(int vectors, int nv) { return ((vectors + nv - 1) / nv + 31) / 3
 
 int parts(int T, int num_sms) { return std::max(1, std::min(T, kMaxParts * num_sms)); }
 
-template <typename X, typename Y>
-cudaError_t forward(const LayerNormOp& p, cudaStream_t s) {
-  const int vec = vector_width(p, sizeof(X), sizeof(Y)), n = p.d / vec;
-  if (n <= 2 * kMaxThreads) {
-    if (vec == 4) layernorm_row_kernel<X, Y, 4, 2><<<p.T, row_threads(n, 2), 0, s>>>(p);
-    else layernorm_row_kernel<X, Y, 1, 2><<<p.T, row_threads(n, 2), 0, s>>>(p);
-  } else if (n <= 4 * kMaxThreads) {
-    if (vec == 4) layernorm_row_kernel<X, Y, 4, 4><<<p.T, row_threads(n, 4), 0, s>>>(p);
-    else layernorm_row_kernel<X, Y, 1, 4><<<p.T, row_threads(n, 4), 0, s>>>(p);
-  } else {
-    layernorm_wide_kernel<X, Y><<<p.T, kMaxThreads, 0, s>>>(p);
-  }
+// Blocks of a row kernel that fit the GPU at once, at most one per row.
+template <typename K>
+int resident(K kernel, const LayerNormOp& p, int threads, int most) {
+  int per_sm = 0;
+  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, threads, 0) != cudaSuccess) return 0;
+  return std::max(1, std::min(p.T, std::min(per_sm, most) * p.num_sms));
+}
+
+template <typename X, typename Y, int VEC, int NV>
+cudaError_t forward_rows(const LayerNormOp& p, int n, cudaStream_t s) {
+  const int threads = row_threads(n, NV), blocks = resident(layernorm_row_kernel<X, Y, VEC, NV>, p, threads, 32);
+  if (blocks == 0) return cudaErrorInvalidConfiguration;
+  layernorm_row_kernel<X, Y, VEC, NV><<<blocks, threads, 0, s>>>(p);
   return cudaGetLastError();
 }
 
+template <typename X, typename Y>
+cudaError_t forward(const LayerNormOp& p, cudaStream_t s) {
+  const int vec = vector_width(p, sizeof(X), sizeof(Y)), n = p.d / vec;
+  if (n <= 2 * kMaxThreads) return vec == 4 ? forward_rows<X, Y, 4, 2>(p, n, s) : forward_rows<X, Y, 1, 2>(p, n, s);
+  if (n <= 4 * kMaxThreads) return vec == 4 ? forward_rows<X, Y, 4, 4>(p, n, s) : forward_rows<X, Y, 1, 4>(p, n, s);
+  layernorm_wide_kernel<X, Y><<<p.T, kMaxThreads, 0, s>>>(p);
+  return cudaGetLastError();
+}
+
+// Up to this many elements the second launch costs more than reading the rows twice (2 M: in L2).
+constexpr int64_t kSmallElements = 2 << 20;
+
 template <typename X, typename Y, int VEC, int NV, bool RES>
-int launch_rows(const LayerNormOp& p, int n, cudaStream_t s) {
+cudaError_t backward_rows(const LayerNormOp& p, int n, cudaStream_t s) {
+  if (p.T > 0 && static_cast<int64_t>(p.T) * p.d <= kSmallElements) {
+    // At least 256 threads, for the blocks of columns.
+    const int threads = std::max(256, row_threads(n, NV));
+    layernorm_backward_kernel<X, Y, VEC, NV, RES, true><<<p.T + (p.d + 31) / 32, threads, 0, s>>>(p, p.T);
+    return cudaGetLastError();
+  }
   const int threads = row_threads(n, NV);
-  int per_sm = 0;
-  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, layernorm_backward_kernel<X, Y, VEC, NV, RES>, threads, 0) !=
-      cudaSuccess)
-    return 0;
-  const int blocks = std::max(1, std::min(p.T, std::min(per_sm, kMaxParts) * p.num_sms));
-  layernorm_backward_kernel<X, Y, VEC, NV, RES><<<blocks, threads, 0, s>>>(p);
-  return blocks;
+  const int blocks = resident(layernorm_backward_kernel<X, Y, VEC, NV, RES, false>, p, threads, kMaxParts);
+  if (blocks == 0) return cudaErrorInvalidConfiguration;
+  layernorm_backward_kernel<X, Y, VEC, NV, RES, false><<<blocks, threads, 0, s>>>(p, blocks);
+  layernorm_reduce_kernel<<<(2 * p.d + 15) / 16, 512, 0, s>>>(p.workspace, blocks, p.d, p.dw, p.db);
+  return cudaGetLastError();
 }
 
 template <typename X, typename Y, bool RES>
-int backward_rows(const LayerNormOp& p, cudaStream_t s) {
+cudaError_t backward_by_size(const LayerNormOp& p, cudaStream_t s) {
   const int vec = vector_width(p, sizeof(X), sizeof(Y)), n = p.d / vec;
   if (n <= 2 * kMaxThreads)
-    return vec == 4 ? launch_rows<X, Y, 4, 2, RES>(p, n, s) : launch_rows<X, Y, 1, 2, RES>(p, n, s);
+    return vec == 4 ? backward_rows<X, Y, 4, 2, RES>(p, n, s) : backward_rows<X, Y, 1, 2, RES>(p, n, s);
   if (n <= 4 * kMaxThreads)
-    return vec == 4 ? launch_rows<X, Y, 4, 4, RES>(p, n, s) : launch_rows<X, Y, 1, 4, RES>(p, n, s);
+    return vec == 4 ? backward_rows<X, Y, 4, 4, RES>(p, n, s) : backward_rows<X, Y, 1, 4, RES>(p, n, s);
   const int blocks = parts(p.T, p.num_sms);
   if (p.T > 0) layernorm_wide_dx_kernel<X, Y><<<p.T, kMaxThreads, 0, s>>>(p);
   layernorm_wide_dw_kernel<X, Y><<<dim3((p.d + kMaxThreads - 1) / kMaxThreads, blocks), kMaxThreads, 0, s>>>(p);
-  return blocks;
+  layernorm_reduce_kernel<<<(2 * p.d + 15) / 16, 512, 0, s>>>(p.workspace, blocks, p.d, p.dw, p.db);
+  return cudaGetLastError();
 }
 
 template <typename X, typename Y>
 cudaError_t backward(const LayerNormOp& p, cudaStream_t s) {
-  const int n = p.dres ? backward_rows<X, Y, true>(p, s) : backward_rows<X, Y, false>(p, s);
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess || n == 0) return e != cudaSuccess ? e : cudaErrorInvalidConfiguration;
-  layernorm_reduce_kernel<<<(2 * p.d + 31) / 32, 1024, 0, s>>>(p.workspace, n, p.d, p.dw, p.db);
-  return cudaGetLastError();
+  return p.dres ? backward_by_size<X, Y, true>(p, s) : backward_by_size<X, Y, false>(p, s);
 }
 
 template <typename X>
