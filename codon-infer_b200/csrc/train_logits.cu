@@ -97,6 +97,32 @@ __global__ void __launch_bounds__(128) logprobs_quad_kernel(const LogitsOp p) {
   uint32_t key[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) key[i] = r.q + 4 * i < p.V ? order_key(v[i]) : 0u;
+  if (p.k > N + N / 4) {  // many: every element's rank, by comparing it with all the others
+    int rank[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) rank[j] = 0;
+#pragma unroll 1
+    for (int o = 0; o < 4; ++o) {
+      const uint32_t before = o < r.q;  // a lane's elements j are in front of those of later lanes
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const uint32_t other = __shfl_sync(0xffffffffu, key[i], o, 4);
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          if (i < j) rank[j] += other >= key[j];
+          else if (i > j) rank[j] += other > key[j];
+          else rank[j] += other > key[j] - before;
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (r.real && r.q + 4 * j < p.V && rank[j] < p.k) {
+        p.top_ids[r.t * p.k + rank[j]] = none ? -1 : r.q + 4 * j;
+        p.top_logp[r.t * p.k + rank[j]] = none ? NAN : v[j] - m - log_s;
+      }
+    return;
+  }
   for (int i = 0; i < p.k; ++i) {
     uint32_t best = 0;
     int id = r.q;
@@ -555,7 +581,9 @@ __global__ void __launch_bounds__(NT) distill_backward_row_kernel(const LogitsOp
 unsigned quads(const LogitsOp& p) { return (static_cast<unsigned>(p.T) + 31) / 32; }
 
 // Threads of a row's block: one warp for short rows; for long ones 512, or 256 where there are more rows than
-// 512-thread blocks fit the GPU at once (4 x 148; 1021 rows of 32003: loss 27 -> 20 us, but 512 of 32768: 32 us).
+// 512-thread blocks fit the GPU at once (4 x 148). Loss of 1021 x 32003 fp16: 20 us with 256, 27 us with 512. What
+// bounds these is the latency of a row's passes: copying rows to shared memory in bulk, or starting from the
+// maximum of a row's first vectors so that the running maximum seldom rises, was no faster.
 int row_block(const LogitsOp& p) {
   if (p.V <= 1024) return 32;
   if (p.V <= 4096) return 128;
