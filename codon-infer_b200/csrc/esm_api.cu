@@ -2175,4 +2175,77 @@ int esm_distill_backward(esm_ctx* c, int32_t type, const void* d_logits, int64_t
   return ESM_OK;
 }
 
+int esm_score(esm_ctx* c, const int32_t* tokens, const int32_t* lengths, int32_t B, int32_t Lmax, const int32_t* targets,
+              int32_t k, float* logp, float* entropy, int32_t* top_ids, float* top_logp) {
+  if (!c || !tokens || !lengths || !logp) return fail(c, ESM_EINVAL, "null argument");
+  std::lock_guard<std::mutex> lk(c->mu);
+  if (B <= 0 || Lmax <= 0) return fail(c, ESM_EINVAL, "empty batch");
+  std::vector<int32_t> cu(B + 1, 0);
+  for (int b = 0; b < B; ++b) {
+    if (lengths[b] <= 0 || lengths[b] > Lmax) return fail(c, ESM_EINVAL, "length outside [1, Lmax]");
+    cu[b + 1] = cu[b] + lengths[b];
+  }
+  int rc = validate_call(c, cu.data(), B, false);
+  if (rc) return rc;
+  const int V = c->cfg.vocab_size, T = cu[B];
+  rc = check_logits(c, ESM_F32, T, V, k, 0);
+  if (rc) return rc;
+  if (k > 0 && (!top_ids || !top_logp)) return fail(c, ESM_EINVAL, "null argument");
+  ESM_CUDA(cudaSetDevice(c->device));
+  cudaStream_t s = c->stream;
+  // Packed on the host (only real tokens cross the bus), and in the forward's output staging on the device:
+  // targets, then logp, entropy, top_ids, top_logp.
+  const size_t row = 3 + 2 * static_cast<size_t>(k), need = T * row;
+  if (need > c->padded_out_cap) {
+    if (c->d_padded_out) cudaFree(c->d_padded_out);
+    c->d_padded_out = nullptr;
+    c->padded_out_cap = 0;
+    ESM_CUDA(cudaMalloc(&c->d_padded_out, need * sizeof(float)));
+    c->padded_out_cap = need;
+  }
+  std::vector<int32_t> packed(T), wanted(T);
+  for (int b = 0; b < B; ++b) {
+    std::copy_n(tokens + static_cast<size_t>(b) * Lmax, lengths[b], packed.begin() + cu[b]);
+    std::copy_n((targets ? targets : tokens) + static_cast<size_t>(b) * Lmax, lengths[b], wanted.begin() + cu[b]);
+  }
+  int32_t* d_targets = reinterpret_cast<int32_t*>(c->d_padded_out);
+  float* d_logp = c->d_padded_out + T;
+  ESM_CUDA(cudaMemcpyAsync(c->tokens, packed.data(), T * sizeof(int32_t), cudaMemcpyHostToDevice, s));
+  ESM_CUDA(cudaMemcpyAsync(d_targets, wanted.data(), T * sizeof(int32_t), cudaMemcpyHostToDevice, s));
+  rc = forward_impl(c, c->tokens, cu.data(), B, c->logits, nullptr, nullptr, nullptr, s);
+  if (rc) return rc;
+  esm::LogitsOp p{};
+  p.dtype = ESM_F32;
+  p.logits = c->logits;
+  p.ld = V;
+  p.T = T;
+  p.V = V;
+  p.k = k;
+  p.targets = d_targets;
+  p.logp = d_logp;
+  p.entropy = d_logp + T;
+  p.top_ids = reinterpret_cast<int32_t*>(d_logp + 2 * static_cast<size_t>(T));
+  p.top_logp = d_logp + (2 + static_cast<size_t>(k)) * T;
+  ESM_CUDA(esm::launch_token_logprobs(p, s));
+  std::vector<float> out(T * (row - 1));
+  ESM_CUDA(cudaMemcpyAsync(out.data(), d_logp, out.size() * sizeof(float), cudaMemcpyDeviceToHost, s));
+  ESM_CUDA(cudaStreamSynchronize(s));
+  const size_t places = static_cast<size_t>(B) * Lmax;
+  std::fill_n(logp, places, 0.0f);
+  if (entropy) std::fill_n(entropy, places, 0.0f);
+  std::fill_n(top_ids, places * k, -1);
+  std::fill_n(top_logp, places * k, 0.0f);
+  const float* ids = out.data() + 2 * static_cast<size_t>(T);
+  for (int b = 0; b < B; ++b) {
+    const size_t to = static_cast<size_t>(b) * Lmax, from = cu[b], n = lengths[b];
+    std::copy_n(out.data() + from, n, logp + to);
+    if (entropy) std::copy_n(out.data() + T + from, n, entropy + to);
+    if (k > 0) {
+      std::memcpy(top_ids + to * k, ids + from * k, n * k * sizeof(int32_t));
+      std::copy_n(ids + static_cast<size_t>(T) * k + from * k, n * k, top_logp + to * k);
+    }
+  }
+  return check_device_word(c);
+}
+
 }  // extern "C"

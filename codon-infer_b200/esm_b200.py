@@ -144,6 +144,7 @@ def lib() -> ctypes.CDLL:
             "esm_layernorm_backward_workspace": [vp, i32, i32, vp],
             "esm_layernorm_backward": [vp, i32, i32, vp, vp, vp, vp, vp, vp, i32, i32, vp, vp, vp, vp, sz, vp],
             "esm_token_logprobs": [vp, i32, vp, i64, i32, i32, vp, i32, vp, vp, vp, vp, vp],
+            "esm_score": [vp, vp, vp, i32, i32, vp, i32, vp, vp, vp, vp],
             "esm_distill_loss": [vp, i32, vp, i64, i32, i32, vp, vp, i32, f32, vp, vp, vp],
             "esm_distill_backward": [vp, i32, vp, i64, i32, i32, vp, vp, i32, f32, vp, vp, vp, i64, vp],
             "esm_check_device": [vp],
@@ -616,6 +617,34 @@ class Model:
                                       _flat(top_ids, "top_ids", (T, k), -1), _flat(top_logp, "top_logp", (T, k)),
                                       _stream(stream))
         self._chk(rc, "esm_token_logprobs")
+
+    def score(self, seqs, targets=None, k: int = 0) -> dict:
+        """The forward and token_logprobs of its logits in one call, from host memory (esm_score): `seqs`
+        is a list of int token arrays, `targets` the tokens to score at every position (default: the
+        sequences' own). Returns padded "logp" and "entropy" [B, Lmax] and, for k > 0, "top_ids" and
+        "top_logp" [B, Lmax, k]."""
+        if k < 0 or k > MAX_ALTERNATIVES:
+            _bad(f"k must be in [0, {MAX_ALTERNATIVES}]")
+        lengths = np.array([len(x) for x in seqs], dtype=np.int32)
+        B, Lmax = len(seqs), int(lengths.max())
+
+        def padded(rows):
+            out = np.zeros((B, Lmax), dtype=np.int32)
+            for i, x in enumerate(rows):
+                out[i, : len(x)] = x
+            return out
+
+        if targets is not None and [len(x) for x in targets] != lengths.tolist():
+            _bad("targets must be as long as the sequences")
+        tokens, wanted = padded(seqs), None if targets is None else padded(targets)
+        logp, entropy = np.empty((B, Lmax), dtype=np.float32), np.empty((B, Lmax), dtype=np.float32)
+        ids, top = np.empty((B, Lmax, k), dtype=np.int32), np.empty((B, Lmax, k), dtype=np.float32)
+        self._chk(lib().esm_score(self._ctx, _p(tokens), _p(lengths), B, Lmax, _p(wanted), k, _p(logp), _p(entropy),
+                                  _p(ids) if k else None, _p(top) if k else None), "esm_score")
+        res = {"logp": logp, "entropy": entropy, "lengths": lengths}
+        if k:
+            res.update(top_ids=ids, top_logp=top)
+        return res
 
     def distill_loss(self, logits, top_ids, top_logits, loss, lse, temperature: float = 1.0, stream=None) -> None:
         """loss [T] of the student's logits [T, V] against a teacher's alternatives top_ids (int32) and

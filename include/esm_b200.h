@@ -330,6 +330,15 @@ int esm_token_logprobs(esm_ctx* ctx, int32_t type, const void* d_logits, int64_t
                        const int32_t* d_targets, int32_t k, float* d_logp, float* d_entropy, int32_t* d_top_ids,
                        float* d_top_logp, void* stream);
 
+/* The forward of esm_forward followed by esm_token_logprobs on its logits, from HOST buffers: what scoring
+ * sequences, or preparing a teacher's alternatives for distillation, needs, without the logits leaving
+ * the GPU. tokens [B, Lmax] and lengths as in esm_forward; targets [B, Lmax], or NULL for the tokens
+ * themselves; logp, entropy (or NULL) [B, Lmax]; top_ids, top_logp [B, Lmax, k] (NULL when k = 0).
+ * Padding positions get 0, and top ids of -1. Positions are not masked: mask them in `tokens` and name
+ * the masked tokens in `targets` for pseudo-likelihoods. */
+int esm_score(esm_ctx* ctx, const int32_t* tokens, const int32_t* lengths, int32_t B, int32_t Lmax,
+              const int32_t* targets, int32_t k, float* logp, float* entropy, int32_t* top_ids, float* top_logp);
+
 /* Distillation loss of T rows of student logits [T, V] against a teacher's alternatives, k per row
  * (esm_token_logprobs' d_top_ids and d_top_logp of the teacher, or its logits at those ids): with
  * q = softmax(logits / temperature) over the vocabulary and p = softmax(top_logits / temperature) over

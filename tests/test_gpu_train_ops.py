@@ -655,6 +655,36 @@ def test_logprobs_row_strides_and_optional_outputs(m, esm):
     m.token_logprobs(torch.empty(0, 33, device="cuda"), entropy=torch.empty(0, device="cuda"))
 
 
+def test_score_is_the_forward_and_its_log_probabilities(esm):
+    cfg = esm.EsmConfig(320, 1280, 1, 20, 33, 64, 0)
+    model = esm.Model(0)
+    model.load_tensors(cfg, esm.DTYPE_FP32, esm.synth_fp32_tensors(cfg, seed=3))
+    model.reserve(200, 4, 64)
+    seqs = [np.arange(n, dtype=np.int32) % 20 + 4 for n in (50, 1, 64, 17)]
+    logits = model.forward(seqs)["logits"]
+    targets = [(x * 7 + 3) % 35 - 1 for x in seqs]           # some outside the vocabulary
+    for want, k in ((None, 0), (targets, 5)):
+        got = model.score(seqs, want, k)
+        for i, x in enumerate(seqs):
+            n = len(x)
+            row = torch.from_numpy(logits[i, :n]).cuda()
+            t = torch.from_numpy((x if want is None else want[i]).astype(np.int32)).cuda()
+            ids = torch.from_numpy(got["top_ids"][i, :n]).cuda() if k else torch.empty(n, 0, dtype=torch.int32, device="cuda")
+            top = torch.from_numpy(got["top_logp"][i, :n]).cuda() if k else torch.empty(n, 0, device="cuda")
+            check_logprobs(row, t, torch.from_numpy(got["logp"][i, :n]).cuda(), torch.from_numpy(got["entropy"][i, :n]).cuda(), ids, top)
+            assert (got["logp"][i, n:] == 0).all() and (got["entropy"][i, n:] == 0).all()
+            assert not k or ((got["top_ids"][i, n:] == -1).all() and (got["top_logp"][i, n:] == 0).all())
+    for bad in ({"k": 34}, {"k": -1}, {"targets": targets[:3]}):
+        with pytest.raises(esm.EsmError) as e:
+            model.score(seqs, **bad)
+        assert e.value.code == esm.ESM_EINVAL
+    model.close()
+    empty = esm.Model(0)
+    with pytest.raises(esm.EsmError, match="no weights"):
+        empty.score(seqs)
+    empty.close()
+
+
 # ---- distillation -----------------------------------------------------------------------------------
 
 def distill_inputs(T, V, k, kind, seed):
