@@ -336,15 +336,7 @@ __device__ __forceinline__ void tmem_ld_wait_regs(uint32_t (&r)[32]) {
                : "memory");
 }
 
-// The same for one and for two loads of 16 columns.
-__device__ __forceinline__ void tmem_ld_wait_regs(uint32_t (&a)[16]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+r"(a[0]), "+r"(a[1]), "+r"(a[2]), "+r"(a[3]), "+r"(a[4]), "+r"(a[5]), "+r"(a[6]), "+r"(a[7]),
-                 "+r"(a[8]), "+r"(a[9]), "+r"(a[10]), "+r"(a[11]), "+r"(a[12]), "+r"(a[13]), "+r"(a[14]),
-                 "+r"(a[15])
-               :
-               : "memory");
-}
+// The same for two loads of 16 columns.
 __device__ __forceinline__ void tmem_ld_wait_regs(uint32_t (&a)[16], uint32_t (&b)[16]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;"
                : "+r"(a[0]), "+r"(a[1]), "+r"(a[2]), "+r"(a[3]), "+r"(a[4]), "+r"(a[5]), "+r"(a[6]), "+r"(a[7]),
@@ -479,8 +471,6 @@ __device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, ui
 constexpr uint32_t kSw128DescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
 // The 64-byte-swizzle layouts (SBO 512 bytes, layout type 4) share the same low-word form.
 constexpr uint32_t kSw64DescHi = (512u >> 4) | (1u << 14) | (4u << 29);
-// K-major rows of one K step (32 bytes) with the 32-byte swizzle (8-row groups 256 bytes apart).
-constexpr uint32_t kSw32DescHi = (256u >> 4) | (1u << 14) | (6u << 29);
 __device__ __forceinline__ uint32_t umma_sw128_lo(uint32_t saddr) { return ((saddr & 0x3FFFFu) >> 4) | (1u << 16); }
 template <uint32_t HI = kSw128DescHi>
 __device__ __forceinline__ void umma_f16_lo(uint32_t tmem_d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc,
@@ -514,49 +504,6 @@ __device__ __forceinline__ void umma_f16_ts_lo(uint32_t tmem_d, uint32_t tmem_a,
 __device__ __forceinline__ void umma_commit_addr(uint32_t bar_saddr) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar_saddr)
                : "memory");
-}
-
-// The same for a whole warp, issued by the lane whose `lead` is not 0.
-template <uint32_t HI>
-__device__ __forceinline__ void umma_f16_lo_if(uint32_t lead, uint32_t tmem_d, uint32_t a_lo, uint32_t b_lo,
-                                               uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n"
-      ".reg .pred p, q;\n"
-      ".reg .b64 ad, bd;\n"
-      "mov.b64 ad, {%1, %5};\n"
-      "mov.b64 bd, {%2, %5};\n"
-      "setp.ne.b32 p, %4, 0;\n"
-      "setp.ne.b32 q, %6, 0;\n"
-      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], ad, bd, %3, p;\n"
-      "}\n" ::"r"(tmem_d),
-      "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(HI), "r"(lead)
-      : "memory");
-}
-template <uint32_t HI>
-__device__ __forceinline__ void umma_f16_ts_lo_if(uint32_t lead, uint32_t tmem_d, uint32_t tmem_a, uint32_t b_lo,
-                                                  uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n"
-      ".reg .pred p, q;\n"
-      ".reg .b64 bd;\n"
-      "mov.b64 bd, {%2, %5};\n"
-      "setp.ne.b32 p, %4, 0;\n"
-      "setp.ne.b32 q, %6, 0;\n"
-      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], bd, %3, p;\n"
-      "}\n" ::"r"(tmem_d),
-      "r"(tmem_a), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(HI), "r"(lead)
-      : "memory");
-}
-__device__ __forceinline__ void umma_commit_if(uint32_t lead, uint32_t bar_saddr) {
-  asm volatile(
-      "{\n"
-      ".reg .pred q;\n"
-      "setp.ne.b32 q, %1, 0;\n"
-      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n"
-      "}\n" ::"r"(bar_saddr),
-      "r"(lead)
-      : "memory");
 }
 
 // ---- clusters and the CTA pair (cta_group::2) ----------------------------------------------------
