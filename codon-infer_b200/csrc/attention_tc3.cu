@@ -150,6 +150,7 @@ __global__ void __launch_bounds__(kThreads3, 2)
 
   if (warp == 8) {
     // ---------------- TMA producer ----------------
+    bool ok = true;
     if (elect_one_sync()) {
       tma_prefetch_desc(&tmap_q);
       tma_prefetch_desc(&tmap_kv);
@@ -164,7 +165,6 @@ __global__ void __launch_bounds__(kThreads3, 2)
           tma_load_2d(smem + t * kQBytes, &tmap_q, q_full, h * kD, start + q0 + t * kQ, pol);
         }
       }
-      bool ok = true;
       int j = 0;
       for (; j < nkv; ++j) {
         const int st = j % kStages3;
@@ -173,20 +173,11 @@ __global__ void __launch_bounds__(kThreads3, 2)
           break;
         }
         uint8_t* dst = smem + kOffKV + st * G::kStageTiles * kKVBytes;
-        const int kept = len - j * kKV;  // keys of this tile inside the sequence
         if constexpr (OP) {
-          if (kept < kKV) {  // the last tile: its V rows past the end are cleared before it is handed on
+          if (len - j * kKV < kKV) {  // the last tile, handed on below
             mbar_arrive_expect_tx(tail, 2 * kKVBytes);
             tma_load_3d(dst, &tmap_kv, tail, 0, p.H + h, start + j * kKV, pol);
             tma_load_3d(dst + kKVBytes, &tmap_kv, tail, 0, 2 * p.H + h, start + j * kKV, pol);
-            if (!mbar_wait(tail, 0, p.err, kDevTimeoutProducer)) {
-              ok = false;
-              break;
-            }
-            uint4* v = reinterpret_cast<uint4*>(dst + kKVBytes + kept * kD * 2);  // rows are whole under the swizzle
-            for (int i = 0; i < (kKV - kept) * kD * 2 / 16; ++i) v[i] = make_uint4(0u, 0u, 0u, 0u);
-            fence_proxy_async_smem();
-            mbar_arrive(&kv_full[st]);
             continue;
           }
         }
@@ -205,6 +196,17 @@ __global__ void __launch_bounds__(kThreads3, 2)
         mbar_wait(q_full, 0, p.err, kDevTimeoutProducer);
         for (int jj = (j - kStages3 > 0 ? j - kStages3 : 0); jj < j; ++jj)
           mbar_wait(&kv_full[jj % kStages3], (jj / kStages3) & 1, p.err, kDevTimeoutProducer);
+      }
+    }
+    if constexpr (OP) {  // a partial last tile's V rows past the end are cleared before it is handed on
+      const int kept = len - (nkv - 1) * kKV, st = (nkv - 1) % kStages3;
+      if (__all_sync(0xffffffffu, ok) && kept < kKV &&
+          __all_sync(0xffffffffu, mbar_wait(tail, 0, p.err, kDevTimeoutProducer))) {
+        uint4* v = reinterpret_cast<uint4*>(smem + kOffKV + st * G::kStageTiles * kKVBytes + kKVBytes + kept * kD * 2);  // rows are whole under the swizzle
+        for (int i = lane; i < (kKV - kept) * kD * 2 / 16; i += 32) v[i] = make_uint4(0u, 0u, 0u, 0u);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&kv_full[st]);
       }
     }
   } else if (warp == 9 || warp == 10) {

@@ -62,7 +62,7 @@ constexpr int kWarpCols = 4 * kStep / kTeamWarps;  // columns of an elementwise 
 constexpr int kStoreWarp = kElemWarps, kLoadWarp = kStoreWarp + 4;
 constexpr int kScoreWarp = kLoadWarp + 1, kProductWarp = kScoreWarp + 1, kSplitWarp = kProductWarp + 1;
 constexpr int kThreads = 32 * (kSplitWarp + 1);
-constexpr int kInfos = 8;      // item records: the producer is at most 5 items ahead of the slowest reader
+constexpr int kInfos = 8;      // item records: the producer writes at most the fifth one after the slowest reader's
 constexpr int kDeltaRows = 64;
 constexpr uint32_t kTmemCols = 512, kColBuf = 128, kColDp = 64, kColAcc1 = 384, kColAcc2 = 448;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -248,7 +248,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int i = 0; i < kInfos; ++i) mbar_init(&info_full[i], 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&own_full[i], 1);
-      mbar_init(&own_empty[i], 1);
+      mbar_init(&own_empty[i], 2);  // the item's scores; its record read by the splitting warp
     }
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&full[i], 2);  // the copies; the parts of lse and D, or for query items the producer again
@@ -476,6 +476,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!mbar_wait_spin(&info_full[item % kInfos], (item / kInfos) & 1, p.err, kDevTimeoutProducer)) break;
       const Item it = *info_at(item);
       if (it.len == 0) break;
+      // Nothing else waits for this warp in query items of whole tiles: the records' ring has to.
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&own_empty[item & 1]);
       const float* lse = p.lse + static_cast<size_t>(it.h) * p.T + it.start;
       const float* delta = p.delta + static_cast<size_t>(it.h) * p.T + it.start;
       float next_l[2], next_d[2];  // of this lane's two rows of the next tile
