@@ -6,7 +6,7 @@
 // are read once. Blocks stay and take every gridDim.x-th row. In the backward pass a block loads its next row
 // before the current one's sums are exchanged, and a thread adds up dw and db of its own columns in
 // registers over all its rows; the blocks' sums go to the workspace and are added there in order by
-// layernorm_reduce_kernel, so the gradients do not depend on timing. Small inputs, which stay in L2, take
+// layernorm_reduce_kernel, so the gradients do not depend on timing. Few rows, which stay in L2, take
 // one launch instead: some blocks compute dx, others read the same rows again for the columns of dw and db.
 // Rows too wide for the registers of a block (kMaxThreads * NV * VEC) take the looping kernels, which read
 // them repeatedly.
@@ -335,12 +335,14 @@ cudaError_t forward(const LayerNormOp& p, cudaStream_t s) {
   return cudaGetLastError();
 }
 
-// Up to this many elements the second launch costs more than reading the rows twice (2 M: in L2).
-constexpr int64_t kSmallElements = 2 << 20;
+// Up to this many rows the second launch costs more than reading the rows twice: a block of columns walks
+// all of them. One launch against two, d = 640 fp32 with fp16 dy: 128 rows 3.0 and 5.0 us, 384 rows 5.3 and
+// 6.1, 512 rows 6.4 and 6.1, 4096 rows 42 and 12; d = 2560: 384 rows 6.6 and 9.0, 1024 rows 13.4 and 11.4.
+constexpr int kSmallRows = 384;
 
 template <typename X, typename Y, int VEC, int NV, bool RES>
 cudaError_t backward_rows(const LayerNormOp& p, int n, cudaStream_t s) {
-  if (p.T > 0 && static_cast<int64_t>(p.T) * p.d <= kSmallElements) {
+  if (p.T > 0 && p.T <= kSmallRows) {
     // At least 256 threads, for the blocks of columns.
     const int threads = std::max(256, row_threads(n, NV));
     layernorm_backward_kernel<X, Y, VEC, NV, RES, true><<<p.T + (p.d + 31) / 32, threads, 0, s>>>(p, p.T);
