@@ -13,6 +13,7 @@
 #include <cstring>
 #include <fstream>
 #include <mutex>
+#include <new>
 #include <string>
 #include <vector>
 
@@ -1856,9 +1857,13 @@ int check_buffers(esm_ctx* c, const Buffer* b, int n, cudaStream_t s) {
   return ESM_OK;
 }
 
+// Limit of row and column counts: indices of a tile or a block behind the last one stay in 32 bits.
+constexpr int32_t kMaxSize = 1 << 30;
+
 int check_attention(esm_ctx* c, int32_t type, int32_t B, int32_t T, int32_t max_len, int32_t H, int32_t dh, float scale) {
   if (type != ESM_F16 && type != ESM_BF16) return fail(c, ESM_EINVAL, "attention takes ESM_F16 or ESM_BF16");
-  if (B < 0 || T < 0 || max_len < 0 || max_len > T) return fail(c, ESM_EINVAL, "attention: bad B, T or max_len");
+  if (B < 0 || T < 0 || T > kMaxSize || max_len < 0 || max_len > T)
+    return fail(c, ESM_EINVAL, "attention: bad B, T or max_len");
   if (H <= 0 || H > 65535 || dh < 8 || dh > 64 || dh % 8)
     return fail(c, ESM_EINVAL, "attention: head_dim must be a multiple of 8 up to 64 and n_heads positive");
   if (!(scale >= 1e-6f && scale <= 1e6f)) return fail(c, ESM_EINVAL, "attention: scale must be in [1e-6, 1e6]");
@@ -1868,7 +1873,7 @@ int check_attention(esm_ctx* c, int32_t type, int32_t B, int32_t T, int32_t max_
 
 int check_logits(esm_ctx* c, int32_t type, int32_t T, int32_t V, int32_t k, int32_t k_min) {
   if (!element_size(type)) return fail(c, ESM_EINVAL, "unknown element type");
-  if (T < 0 || V <= 0) return fail(c, ESM_EINVAL, "bad number of rows or vocabulary size");
+  if (T < 0 || V <= 0 || V > kMaxSize) return fail(c, ESM_EINVAL, "bad number of rows or vocabulary size");
   if (k < k_min || k > ESM_MAX_ALTERNATIVES || k > V)
     return fail(c, ESM_EINVAL, "the number of alternatives must be in [" + std::to_string(k_min) + ", min(vocabulary, " +
                                    std::to_string(ESM_MAX_ALTERNATIVES) + ")]");
@@ -1877,7 +1882,7 @@ int check_logits(esm_ctx* c, int32_t type, int32_t T, int32_t V, int32_t k, int3
 
 int check_layernorm(esm_ctx* c, int32_t x_type, int32_t y_type, int32_t T, int32_t d) {
   if (!element_size(x_type) || !element_size(y_type)) return fail(c, ESM_EINVAL, "unknown element type");
-  if (T < 0 || d <= 0) return fail(c, ESM_EINVAL, "layernorm: bad number of rows or columns");
+  if (T < 0 || d <= 0 || d > kMaxSize / 2) return fail(c, ESM_EINVAL, "layernorm: bad number of rows or columns");
   return ESM_OK;
 }
 
@@ -2105,8 +2110,8 @@ int esm_distill_loss(esm_ctx* c, int32_t type, const void* d_logits, int64_t ld,
   std::lock_guard<std::mutex> lk(c->mu);
   int rc = check_logits(c, type, T, V, k, 1);
   if (rc) return rc;
-  if (!(temperature > 0.0f) || !std::isfinite(temperature))
-    return fail(c, ESM_EINVAL, "distillation: the temperature must be positive and finite");
+  if (!(temperature >= 1e-6f && temperature <= 1e6f))
+    return fail(c, ESM_EINVAL, "distillation: the temperature must be in [1e-6, 1e6]");
   if (T == 0) return ESM_OK;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   DeviceScope dev(c->device);
@@ -2142,8 +2147,8 @@ int esm_distill_backward(esm_ctx* c, int32_t type, const void* d_logits, int64_t
   std::lock_guard<std::mutex> lk(c->mu);
   int rc = check_logits(c, type, T, V, k, 1);
   if (rc) return rc;
-  if (!(temperature > 0.0f) || !std::isfinite(temperature))
-    return fail(c, ESM_EINVAL, "distillation: the temperature must be positive and finite");
+  if (!(temperature >= 1e-6f && temperature <= 1e6f))
+    return fail(c, ESM_EINVAL, "distillation: the temperature must be in [1e-6, 1e6]");
   if (T == 0) return ESM_OK;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   DeviceScope dev(c->device);
@@ -2176,15 +2181,21 @@ int esm_distill_backward(esm_ctx* c, int32_t type, const void* d_logits, int64_t
 }
 
 int esm_score(esm_ctx* c, const int32_t* tokens, const int32_t* lengths, int32_t B, int32_t Lmax, const int32_t* targets,
-              int32_t k, float* logp, float* entropy, int32_t* top_ids, float* top_logp) {
+              int32_t k, float* logp, float* entropy, int32_t* top_ids, float* top_logp) try {
   if (!c || !tokens || !lengths || !logp) return fail(c, ESM_EINVAL, "null argument");
   std::lock_guard<std::mutex> lk(c->mu);
   if (B <= 0 || Lmax <= 0) return fail(c, ESM_EINVAL, "empty batch");
-  std::vector<int32_t> cu(B + 1, 0);
+  int64_t total = 0;
   for (int b = 0; b < B; ++b) {
     if (lengths[b] <= 0 || lengths[b] > Lmax) return fail(c, ESM_EINVAL, "length outside [1, Lmax]");
-    cu[b + 1] = cu[b] + lengths[b];
+    total += lengths[b];
   }
+  if (!c->loaded) return fail(c, ESM_EINVAL, "no weights loaded");
+  if (c->cap_tokens == 0) return fail(c, ESM_EINVAL, "call esm_reserve before the first forward");
+  if (B > c->cap_seqs || total > c->cap_tokens)  // before anything is allocated for them
+    return fail(c, ESM_ECAPACITY, "batch exceeds the reserved number of sequences or tokens");
+  std::vector<int32_t> cu(B + 1, 0);
+  for (int b = 0; b < B; ++b) cu[b + 1] = cu[b] + lengths[b];
   int rc = validate_call(c, cu.data(), B, false);
   if (rc) return rc;
   const int V = c->cfg.vocab_size, T = cu[B];
@@ -2246,6 +2257,8 @@ int esm_score(esm_ctx* c, const int32_t* tokens, const int32_t* lengths, int32_t
     }
   }
   return check_device_word(c);
+} catch (const std::bad_alloc&) {
+  return ESM_ENOMEM;
 }
 
 }  // extern "C"

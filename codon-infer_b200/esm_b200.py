@@ -221,6 +221,13 @@ def _flat(t, name: str, shape: tuple, ty: int = TYPE_F32):
     return t.data_ptr()
 
 
+def _space(t) -> tuple[int, int]:
+    """(pointer, bytes) of a contiguous workspace tensor."""
+    if not t.is_contiguous():
+        _bad("workspace must be contiguous")
+    return t.data_ptr(), t.nbytes
+
+
 def _stream(stream):
     return None if stream is None else (stream if isinstance(stream, int) else stream.cuda_stream)
 
@@ -572,8 +579,8 @@ class Model:
         B = cu_seqlens.shape[0] - 1
         rc = lib().esm_attention_backward(self._ctx, ty, q, ldq, _flat(cu_seqlens, "cu_seqlens", (B + 1,), -1), B, T,
                                           max_len, n_heads, dh, dh ** -0.5 if scale is None else scale, o, ldo,
-                                          _flat(lse, "lse", (n_heads, T)), g, ldg, dq, lddq, workspace.data_ptr(),
-                                          workspace.nbytes, _stream(stream))
+                                          _flat(lse, "lse", (n_heads, T)), g, ldg, dq, lddq, *_space(workspace),
+                                          _stream(stream))
         self._chk(rc, "esm_attention_backward")
 
     def layernorm(self, x, w, b, y, mean=None, rstd=None, eps: float = 1e-5, stream=None) -> None:
@@ -599,8 +606,8 @@ class Model:
         rc = lib().esm_layernorm_backward(self._ctx, xt, yt, _flat(dy, "dy", (T, d), yt), _flat(x, "x", (T, d), xt),
                                           _flat(w, "w", (d,)), _flat(mean, "mean", (T,)), _flat(rstd, "rstd", (T,)),
                                           _flat(dres, "dres", (T, d), xt), T, d, _flat(dx, "dx", (T, d), xt),
-                                          _flat(dw, "dw", (d,)), _flat(db, "db", (d,)), workspace.data_ptr(),
-                                          workspace.nbytes, _stream(stream))
+                                          _flat(dw, "dw", (d,)), _flat(db, "db", (d,)), *_space(workspace),
+                                          _stream(stream))
         self._chk(rc, "esm_layernorm_backward")
 
     def token_logprobs(self, logits, targets=None, logp=None, entropy=None, top_ids=None, top_logp=None,
@@ -625,6 +632,8 @@ class Model:
         "top_logp" [B, Lmax, k]."""
         if k < 0 or k > MAX_ALTERNATIVES:
             _bad(f"k must be in [0, {MAX_ALTERNATIVES}]")
+        if not len(seqs):
+            _bad("score needs at least one sequence")
         lengths = np.array([len(x) for x in seqs], dtype=np.int32)
         B, Lmax = len(seqs), int(lengths.max())
 

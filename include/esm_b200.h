@@ -272,9 +272,9 @@ enum { ESM_F32 = 0, ESM_F16 = 1, ESM_BF16 = 2 };
  * d_qkv [T, 3 H head_dim] of `type` (ESM_F16 or ESM_BF16): queries, keys and values, head h at columns
  * h * head_dim of each part; d_out [T, H head_dim]; both with rows on 16-byte boundaries. d_cu_seqlens
  * [B + 1] (int32, DEVICE memory): sequence b is rows cu[b] .. cu[b + 1], empty ones allowed; max_len
- * bounds their lengths. T is the number of rows of the buffers: rows behind the last sequence are
- * left as they are. head_dim is a multiple of 8 up to 64, scale in [1e-6, 1e6]; B and
- * n_heads are at most 65535. d_lse [H, T] or NULL (the
+ * <= T bounds their lengths (the launch is sized by it, so a close bound is faster). T is the number of
+ * rows of the buffers: rows behind the last sequence are left as they are. head_dim is a multiple of 8
+ * up to 64, scale in [1e-6, 1e6]; B and n_heads are at most 65535, T at most 2^30. d_lse [H, T] or NULL (the
  * backward pass needs it). Scores, sums and outputs are accumulated in fp32, probabilities are rounded to
  * `type` for the product with V. Offsets that do not fit (descending, beyond T or longer than
  * max_len) are noticed on the device: that sequence is skipped and esm_check_device returns
@@ -290,7 +290,8 @@ int esm_attention(esm_ctx* ctx, int32_t type, const void* d_qkv, int64_t ld_qkv,
  *   dS = P (dout V^T - D),  dQ = scale dS K,  dK = scale dS^T Q.
  * P and dS are rounded to `type` for the products; with ESM_F16 each is scaled by a power of two
  * first (from the largest |dout| and |V| of the sequence and head), so small gradients do not
- * underflow. d_workspace: esm_attention_backward_workspace bytes, 16-byte aligned. */
+ * underflow; products q k and sums of dout out beyond 2^30 in magnitude are outside its range.
+ * d_workspace: esm_attention_backward_workspace bytes, 16-byte aligned. */
 int esm_attention_backward_workspace(int32_t B, int32_t T, int32_t n_heads, size_t* bytes);
 int esm_attention_backward(esm_ctx* ctx, int32_t type, const void* d_qkv, int64_t ld_qkv,
                            const int32_t* d_cu_seqlens, int32_t B, int32_t T, int32_t max_len, int32_t n_heads,
@@ -343,7 +344,7 @@ int esm_score(esm_ctx* ctx, const int32_t* tokens, const int32_t* lengths, int32
  * (esm_token_logprobs' d_top_ids and d_top_logp of the teacher, or its logits at those ids): with
  * q = softmax(logits / temperature) over the vocabulary and p = softmax(top_logits / temperature) over
  * the row's alternatives,
- *   loss[t] = temperature^2 sum_i p_i (log p_i - log q[id_i]).
+ *   loss[t] = temperature^2 sum_i p_i (log p_i - log q[id_i]),  temperature in [1e-6, 1e6].
  * An alternative whose id is outside [0, V) is absent, and its d_top_logits entry is ignored; a row
  * without any (or with none above -inf) has loss 0. An id that is given twice counts with both its
  * probabilities. d_lse[t] = log sum_j exp(logits[t, j] / temperature), for the gradient. */

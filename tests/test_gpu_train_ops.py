@@ -893,3 +893,190 @@ def test_a_distillation_step(m):
     for got, ref in zip((dx, dw, db), want):
         assert float((got.double() - ref).norm()) <= rel * float(ref.norm())
     assert float((loss.double() - total.detach()).norm()) <= 3 * 4 * 2.0 ** -11 * float(total.detach().norm())
+
+
+# ---- many sequences, long buffers, graphs and streams -------------------------------------------------
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("length", [1, 64, 128, 40])
+def test_attention_of_many_short_sequences(m, kind, length):
+    """Items of one or two steps, whole and partial tiles, several per block, and empty sequences between."""
+    H, dh, B = 5, 32, 220
+    lens = [length if b % 7 else 0 for b in range(B)]
+    cu, qkv, dout = attention_inputs(lens, H, dh, kind, seed=70 + length)
+    max_len = min(2 * length + 100, qkv.shape[0])   # a loose bound
+    out, lse = run_forward(m, cu, qkv, H, max_len)
+    check_forward(cu, qkv, H, out, lse)
+    check_backward(cu, qkv, H, out, lse, dout, run_backward(m, cu, qkv, H, max_len, out, lse, dout))
+
+
+def test_attention_of_the_most_sequences(m):
+    lens = [0] * 65535
+    for at in (0, 1, 30000, 65533, 65534):
+        lens[at] = 20
+    cu, qkv, dout = attention_inputs(lens, 2, 16, "f16", seed=80)
+    out, lse = run_forward(m, cu, qkv, 2, 100)
+    check_forward(cu, qkv, 2, out, lse)
+    check_backward(cu, qkv, 2, out, lse, dout, run_backward(m, cu, qkv, 2, 100, out, lse, dout))
+
+
+def test_attention_offsets_beyond_32_bits(m):
+    """Rows 800,000 elements apart: the last ones lie more than 2^31 elements into the buffer."""
+    H, dh, T, ld = 2, 64, 2800, 800000
+    d = H * dh
+    assert T * ld > 2 ** 31
+    qkv = torch.empty(T, ld, dtype=torch.float16, device="cuda")[:, :3 * d]
+    dqkv = torch.empty(T, ld, dtype=torch.float16, device="cuda")[:, :3 * d]
+    cu = torch.tensor([0, 2500, 2731, 2800], dtype=torch.int32, device="cuda")
+    qkv.copy_(randn(81, T, 3 * d))
+    dout = (0.05 * randn(82, T, d)).half()
+    out, lse = run_forward(m, cu, qkv, H, 2500)
+    check_forward(cu, qkv.contiguous(), H, out, lse)
+    ws = torch.empty(m.attention_backward_workspace(3, T, H), dtype=torch.uint8, device="cuda")
+    m.attention_backward(qkv, cu, 2500, H, out, lse, dout, dqkv, ws, stream=torch.cuda.current_stream())
+    check_backward(cu, qkv.contiguous(), H, out, lse, dout, dqkv.contiguous())
+
+
+def test_layernorm_offsets_beyond_32_bits(m):
+    T, d = 1_700_001, 1280
+    assert T * d > 2 ** 31
+    gen = torch.Generator(device="cuda").manual_seed(83)
+    x = torch.empty(T, d, dtype=torch.float16, device="cuda").normal_(generator=gen)
+    w, b = 1 + 0.2 * randn(84, d), 0.1 * randn(85, d)
+    y, mean, rstd = run_ln(m, x, w, b, "f16")
+    ends = [slice(0, 100), slice(T - 100, T)]
+    for at in ends:
+        check_ln(x[at], w, b, y[at], mean[at], rstd[at])
+    dy = y
+    dx, dw, db = run_ln_backward(m, dy, x, w, mean, rstd)
+    for at in ends:   # the rows' own gradient; that of the weights is over all of them
+        small = run_ln_backward(m, dy[at], x[at], w, mean[at], rstd[at])
+        check_ln_backward(dy[at], x[at], w, mean[at], rstd[at], None, dx[at], *small[1:])
+    want_w, want_b, size_w, size_b = (torch.zeros(d, dtype=torch.float64, device="cuda") for _ in range(4))
+    for at in range(0, T, 100_000):
+        at = slice(at, at + 100_000)
+        g, xh = dy[at].double(), (x[at].double() - mean[at].double()[:, None]) * rstd[at].double()[:, None]
+        want_b += g.sum(0)
+        size_b += g.abs().sum(0)
+        want_w += (g * xh).sum(0)
+        size_w += (g * xh).abs().sum(0)
+    # At least 148 blocks share the rows, each adding its own up one after another. A term of dw also carries
+    # the rounding of xh, a few E of |x| rstd (rstd and |x| are near 1 here).
+    N = (T / 148 + 64) * E
+    within(dw, want_w, N * size_w + 8 * E * size_b, "dw")
+    within(db, want_b, N * size_b, "db")
+
+
+def test_logits_offsets_beyond_32_bits(m):
+    T, V, ld = 70_000, 33, 32768
+    assert T * ld > 2 ** 31
+    for V in (33, 300):
+        x = torch.empty(T, ld, dtype=torch.float16, device="cuda")[:, :V]
+        dx = torch.empty(T, ld, dtype=torch.float16, device="cuda")[:, :V]
+        small, ids, top, dloss = distill_inputs(T, V, 4, "f16", seed=86)
+        x.copy_(small)
+        targets = ids[:, 0].contiguous()
+        check_logprobs(small, targets, *run_logprobs(m, x, targets, 4))
+        loss, lse = torch.empty(T, device="cuda"), torch.empty(T, device="cuda")
+        m.distill_loss(x, ids, top, loss, lse, stream=torch.cuda.current_stream())
+        m.distill_backward(x, ids, top, lse, dloss, dx, stream=torch.cuda.current_stream())
+        check_distill(small, ids, top, dloss, 1.0, loss, lse, dx)
+
+
+@pytest.mark.parametrize("T, d", [(384, 96), (385, 96), (384, 5121), (385, 5121), (2, 9000), (400, 9000), (3000, 8), (3000, 1)])
+def test_layernorm_few_and_many_rows_and_wide_ones(m, T, d):
+    x, w, b = ln_inputs(T, d, "f32", seed=87)
+    y, mean, rstd = run_ln(m, x, w, b, "bf16")
+    check_ln(x, w, b, y, mean, rstd)
+    dy = (0.05 * randn(88, T, d)).bfloat16()
+    dres = randn(89, T, d)
+    check_ln_backward(dy, x, w, mean, rstd, dres, *run_ln_backward(m, dy, x, w, mean, rstd, dres))
+
+
+def test_rows_operators_in_a_graph(m):
+    """Captured calls answer for what their buffers hold when they are replayed."""
+    for T, d, V in ((40, 64, 33), (900, 320, 3001)):
+        k = 5
+        x, w, b = ln_inputs(T, d, "f32", seed=90)
+        dy = 0.05 * randn(91, T, d)
+        logits, ids, top, dloss = distill_inputs(T, V, k, "f32", seed=92)
+        targets = ids[:, 1].contiguous()
+        buffers = [torch.zeros_like(t) for t in (x, dy, logits, dloss)]
+        got = {}
+        stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+        run_ln(m, x, w, b, "f32")
+        torch.cuda.synchronize()
+
+        def step(x, dy, logits, dloss):
+            y, mean, rstd = run_ln(m, x, w, b, "f32")
+            return (y, mean, rstd, *run_ln_backward(m, dy, x, w, mean, rstd), *run_logprobs(m, logits, targets, k),
+                    *run_distill(m, logits, ids, top, dloss, 2.0))
+
+        with torch.cuda.graph(graph, stream=stream):
+            got = step(*buffers)
+        for buf, t in zip(buffers, (x, dy, logits, dloss)):
+            buf.copy_(t)
+        for _ in range(2):
+            graph.replay()
+        torch.cuda.synchronize()
+        for a, c in zip(got, step(x, dy, logits, dloss)):
+            assert torch.equal(a, c)
+
+
+def test_two_streams_at_once(m):
+    """Calls that run side by side, with a workspace each, do not disturb one another."""
+    H, dh = 4, 32
+    inputs = [attention_inputs([300, 17, 250 + i], H, dh, "f16", seed=93 + i) for i in range(2)]
+    norms = [(*ln_inputs(2000, 320, "f32", seed=95 + i), randn(97 + i, 2000, 320).half()) for i in range(2)]
+
+    def step(i):
+        cu, qkv, dout = inputs[i]
+        out, lse = run_forward(m, cu, qkv, H, 300)
+        x, w, b, dy = norms[i]
+        y, mean, rstd = run_ln(m, x, w, b, "f16")
+        return (out, lse, run_backward(m, cu, qkv, H, 300, out, lse, dout), y, *run_ln_backward(m, dy, x, w, mean, rstd))
+
+    alone = [step(i) for i in range(2)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    together = []
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                together.append((i, step(i)))
+    torch.cuda.synchronize()
+    for i, got in together:
+        for a, c in zip(got, alone[i]):
+            assert torch.equal(a, c)
+
+
+def test_limits_of_sizes_and_temperatures(m, esm):
+    L, big = esm.lib(), 2 ** 30 + 1
+    assert L.esm_token_logprobs(m._ctx, 0, None, big, 5, big, None, 0, None, None, None, None, None) == esm.ESM_EINVAL
+    assert "vocabulary" in L.esm_last_error(m._ctx).decode()
+    assert L.esm_layernorm(m._ctx, 0, 0, None, None, None, 1e-5, 1, big // 2 + 1, None, None, None, None) == esm.ESM_EINVAL
+    assert "columns" in L.esm_last_error(m._ctx).decode()
+    assert L.esm_attention(m._ctx, 1, None, 24, None, 1, big, 5, 1, 8, 1.0, None, 8, None, None) == esm.ESM_EINVAL
+    assert "bad B, T" in L.esm_last_error(m._ctx).decode()
+    x, ids, top, dloss = distill_inputs(4, 33, 3, "f32", seed=99)
+    for tau in (1e-7, 1e7):
+        with pytest.raises(esm.EsmError, match="temperature"):
+            run_distill(m, x, ids, top, dloss, tau)
+
+
+def test_score_refuses_more_than_was_reserved(esm):
+    cfg = esm.EsmConfig(320, 1280, 1, 20, 33, 64, 0)
+    model = esm.Model(0)
+    model.load_tensors(cfg, esm.DTYPE_FP32, esm.synth_fp32_tensors(cfg, seed=3))
+    seq = np.arange(10, dtype=np.int32) + 4
+    with pytest.raises(esm.EsmError, match="esm_reserve"):
+        model.score([seq])
+    model.reserve(25, 3, 12)
+    for seqs in ([seq[:2]] * 4, [seq] * 3, [np.tile(seq, 2)]):   # sequences, tokens, one sequence's length
+        with pytest.raises(esm.EsmError) as e:
+            model.score(seqs)
+        assert e.value.code == esm.ESM_ECAPACITY
+    with pytest.raises(esm.EsmError, match="length outside"):
+        model.score([seq, seq[:0]])
+    assert model.score([seq, seq])["logp"].shape == (2, 10)
+    model.close()

@@ -99,3 +99,18 @@ def test_null_context(esm):
     assert L.esm_attention(None, 1, None, 0, None, 0, 0, 0, 1, 8, 1.0, None, 0, None, None) == esm.ESM_EINVAL
     assert L.esm_layernorm(None, 0, 0, None, None, None, 1e-5, 0, 1, None, None, None, None) == esm.ESM_EINVAL
     assert L.esm_token_logprobs(None, 0, None, 0, 0, 1, None, 0, None, None, None, None, None) == esm.ESM_EINVAL
+
+
+def test_workspaces_are_contiguous(esm, model):
+    """nbytes of an expanded or strided tensor says nothing about the memory behind its pointer."""
+    a = attention_args()
+    for ws in (torch.zeros(1, dtype=torch.uint8).expand(1 << 20), torch.zeros(1 << 16, dtype=torch.uint8)[::2]):
+        refused(esm, model.attention_backward, a["qkv"], a["cu"], 12, 2, a["out"], a["lse"], a["dout"], a["dqkv"], ws,
+                match="workspace must be contiguous")
+        x, w, s = torch.zeros(3, 8), torch.zeros(8), torch.zeros(3)
+        refused(esm, model.layernorm_backward, x, x, w, s, s, x.clone(), w.clone(), w.clone(), ws,
+                match="workspace must be contiguous")
+
+
+def test_score_refuses_an_empty_batch(esm, model):
+    refused(esm, model.score, [], match="at least one sequence")
