@@ -834,10 +834,11 @@ bool make_tmap_op_heads(CUtensorMap* map, const void* base, bool bf16, uint64_t 
   const cuuint64_t strides[2] = {static_cast<cuuint64_t>(head_dim) * 2, ld * 2};
   const cuuint32_t box[3] = {head_dim <= 32 ? 32u : 64u, 1, box_rows};
   const cuuint32_t estr[3] = {1, 1, 1};
+  // A head's row is at most 128 bytes of a caller's row: fetching 256 loads other heads' (DH 32: 5 % slower).
   const CUresult r = enc(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
                          const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                          head_dim <= 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
-                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS;
 }
 

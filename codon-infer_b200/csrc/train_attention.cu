@@ -14,7 +14,7 @@
 //   queries     Q    dO   K    V      S = A1 B1^T, dP = A2 B2^T, acc1 (dQ) += dS B1
 //   keys        K    V    Q    dO     S^T = A1 B1^T, dP^T = A2 B2^T, acc1 (dK) += dS^T B1, acc2 (dV) += P^T B2
 //
-// One persistent block per SM takes every gridDim.x-th item. Tensor memory (512 columns): three score
+// One persistent block per SM takes items from a list (see the producer). Tensor memory (512 columns): three score
 // buffers of 128 columns (S in the first 64, dP in the other 64), acc1 and acc2. Step n uses buffer n % 3, so
 // the tensor cores compute the next steps' scores and the last one's products while the elementwise warps
 // work on a step. P and dS go back over S and dP as 16-bit pairs (each warp over the first half of the 16
@@ -97,6 +97,7 @@ struct BwdParams {
   const float* lse;        // [H, T]
   float* delta;            // [H, T]
   float* peaks;            // fp16: [2][H][blocks], largest |dO| and |V| of each 64 rows
+  unsigned long long* claimed;  // candidates given to blocks; attention_delta_kernel sets it to 0
   int blocks;              // T / 64 + B
   int B, T, max_len, H, dh;
   float scale;
@@ -118,6 +119,7 @@ __device__ __forceinline__ int row_block(int start, int b, int i) { return start
 template <typename E>
 __global__ void __launch_bounds__(256) attention_delta_kernel(const BwdParams p) {
   int start, len;
+  if (threadIdx.x == 0 && blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0) *p.claimed = 0;
   if (!sequence(p, blockIdx.z, &start, &len)) return;
   const int h = blockIdx.y, part = threadIdx.x & 3, i = blockIdx.x * kDeltaRows + (threadIdx.x >> 2);
   if (static_cast<int>(blockIdx.x) * kDeltaRows >= len) return;
@@ -285,29 +287,54 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == kLoadWarp) {
     // ---------------- producer ----------------
     const uint64_t pol = l2_policy_evict_normal();
+    // Candidates are the 128-row blocks of all sequences, for every head (the fastest index: blocks then work on
+    // neighbouring memory; with the heads outermost 16 x 1024 took 4 % longer) and kind (key items, which take
+    // longer, first). A block takes them in batches, one per lane. Where the sequences are about as long as
+    // max_len, each has `tiles` of them and a block takes every gridDim.x-th. Otherwise they are numbered like
+    // row_block's (some numbers have no rows), and with every gridDim.x-th the sum of one block's steps was up to
+    // a third above the mean: only the first batch, 7/8 of an even share, is given like that, and the rest is
+    // claimed from a counter in smaller and smaller batches. 32 x 64..512 tokens, 20 x 24 heads: 117 -> 102 us; 24 x
+    // 30..1022 tokens, 20 x 64: 282 -> 249; 64 x 100 tokens by claims 55 -> 72, hence the rule. A claim takes
+    // about as long as one or two steps of a short sequence, hence `least`.
     const int tiles = (p.max_len + kOwn - 1) / kOwn;
-    const int64_t half = static_cast<int64_t>(tiles) * p.H * p.B, total = 2 * half;
+    const bool even = static_cast<int64_t>(tiles) * p.B <= p.T / kOwn + p.B;
+    const int64_t slots = even ? static_cast<int64_t>(tiles) * p.B : p.T / kOwn + p.B, half = slots * p.H, total = 2 * half;
+    const int64_t least = 1 + static_cast<int64_t>(512) * p.B / p.T;
+    auto share = [&](int64_t left) { return static_cast<int>(min(int64_t(32), max(least, left / gridDim.x))); };
+    int batch = even ? 32 : share(total * 7 / 8);
+    const int64_t handed = static_cast<int64_t>(batch) * gridDim.x;
+    int64_t base = blockIdx.x, stride = gridDim.x;
     bool ok = true;
     int item = 0, n = 0;
     // Loads in flight when a wait gives up must land before the block exits.
     int own_loaded = 0;
-    for (int64_t base = blockIdx.x; base < total && ok; base += static_cast<int64_t>(32) * gridDim.x) {
-      // 32 candidates at a time, one per lane.
-      const int64_t at = base + static_cast<int64_t>(lane) * gridDim.x;
+    while (base < total && ok) {
+      // The next batch is claimed now, so that the counter's latency passes behind this one's items.
+      const int next_batch = share((total - max(base, handed)) / 4);
+      unsigned long long next = 0;
+      if (lane == 0 && !even && handed < total) next = atomicAdd(p.claimed, static_cast<unsigned long long>(next_batch));
+      const int64_t at = base + lane * stride;
       Item it{};
-      if (at < total) {
+      if (lane < batch && at < total) {
         const int64_t r = at < half ? at : at - half;
+        const int slot = static_cast<int>(r / p.H);
         it.keys = at < half;
-        it.r0 = static_cast<int>(r % tiles) * kOwn;
-        it.h = static_cast<int>(r / tiles % p.H);
-        const int b = static_cast<int>(r / tiles / p.H);
+        it.h = static_cast<int>(r % p.H);
+        int b = even ? slot / tiles : 0;
+        for (int left = even ? 1 : p.B; left > 1;) {  // the last sequence whose first block is not behind the slot
+          const int upper = left / 2;
+          if (p.cu[b + upper] / kOwn + b + upper <= slot) {
+            b += upper;
+            left -= upper;
+          } else {
+            left = upper;
+          }
+        }
         it.start = p.cu[b];
         it.len = p.cu[b + 1] - it.start;
-        if (!packed_rows(it.start, it.len, p.T, p.max_len)) {
-          atomicOr(p.err, kDevBadSeqlens);
-          it.len = 0;
-        }
-        if (it.r0 >= it.len) it.len = 0;
+        const int i = even ? slot % tiles : slot - (it.start / kOwn + b);
+        it.r0 = i * kOwn;
+        if (!packed_rows(it.start, it.len, p.T, p.max_len) || i < 0 || i >= (it.len + kOwn - 1) / kOwn) it.len = 0;
         if (it.len > 0) it.ds_exp = ds_exponent<E>(p, it.start, it.len, b, it.h);
       }
       for (uint32_t found = __ballot_sync(0xffffffffu, it.len > 0); found != 0 && ok; found &= found - 1) {
@@ -353,6 +380,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         ok = __shfl_sync(0xffffffffu, ok, 0);
         ++item;
       }
+      if (even) {
+        base += 32 * stride;
+        continue;
+      }
+      if (handed >= total) break;
+      base = handed + static_cast<int64_t>(__shfl_sync(0xffffffffu, next, 0));
+      batch = next_batch;
+      stride = 1;
     }
     if (ok) {
       ok = mbar_wait(&own_empty[item & 1], ((item >> 1) & 1) ^ 1u, p.err, kDevTimeoutProducer);  // the record is free
@@ -699,7 +734,7 @@ cudaError_t backward(const AttnOp& a, const BwdParams& p, cudaStream_t s) {
   cudaError_t e = allow_smem(attention_backward_kernel<DH, E>, Bwd<DH>::kSmem, configured);
   if (e != cudaSuccess) return e;
   attention_delta_kernel<E><<<dim3((a.max_len + kDeltaRows - 1) / kDeltaRows, a.H, a.B), 256, 0, s>>>(p);
-  const int64_t items = static_cast<int64_t>(2) * ((a.max_len + kOwn - 1) / kOwn) * a.H * a.B;
+  const int64_t items = static_cast<int64_t>(2) * (a.T / kOwn + a.B) * a.H;  // at most
   attention_backward_kernel<DH, E>
       <<<static_cast<unsigned>(std::min<int64_t>(items, a.num_sms)), kThreads, Bwd<DH>::kSmem, s>>>(tm_qkv, tm_dout, tm_qkv_own,
                                                                                                    tm_dout_own, p);
@@ -709,7 +744,7 @@ cudaError_t backward(const AttnOp& a, const BwdParams& p, cudaStream_t s) {
 }  // namespace
 
 size_t attention_backward_bytes(int B, int T, int H) {
-  return static_cast<size_t>(H) * T * 4 + static_cast<size_t>(H) * (T / kDeltaRows + B) * 8;
+  return sizeof(unsigned long long) + static_cast<size_t>(H) * T * 4 + static_cast<size_t>(H) * (T / kDeltaRows + B) * 8;
 }
 
 cudaError_t launch_attention_backward(const AttnOp& a, cudaStream_t s) {
@@ -724,8 +759,9 @@ cudaError_t launch_attention_backward(const AttnOp& a, cudaStream_t s) {
   p.ld_dqkv = a.ld_dqkv;
   p.cu = a.cu;
   p.lse = a.lse;
-  p.delta = a.workspace;
-  p.peaks = a.workspace + static_cast<size_t>(a.H) * a.T;
+  p.claimed = reinterpret_cast<unsigned long long*>(a.workspace);
+  p.delta = a.workspace + 2;
+  p.peaks = p.delta + static_cast<size_t>(a.H) * a.T;
   p.blocks = a.T / kDeltaRows + a.B;
   p.B = a.B;
   p.T = a.T;

@@ -277,8 +277,8 @@ enum { ESM_F32 = 0, ESM_F16 = 1, ESM_BF16 = 2 };
  * up to 64, scale in [1e-6, 1e6]; B and n_heads are at most 65535, T at most 2^30. d_lse [H, T] or NULL (the
  * backward pass needs it). Scores, sums and outputs are accumulated in fp32, probabilities are rounded to
  * `type` for the product with V. Offsets that do not fit (descending, beyond T or longer than
- * max_len) are noticed on the device: that sequence is skipped and esm_check_device returns
- * ESM_EINVAL. */
+ * max_len) are noticed on the device: that sequence, and in the backward pass perhaps others, is skipped and
+ * esm_check_device returns ESM_EINVAL. */
 int esm_attention(esm_ctx* ctx, int32_t type, const void* d_qkv, int64_t ld_qkv, const int32_t* d_cu_seqlens,
                   int32_t B, int32_t T, int32_t max_len, int32_t n_heads, int32_t head_dim, float scale, void* d_out,
                   int64_t ld_out, float* d_lse, void* stream);
