@@ -343,7 +343,7 @@ __global__ void __launch_bounds__(kThreads3, 2)
             for (int i = 0; i < 16; ++i) {
               float a0, a1;
               f2_unpack(f2_fma(f2_pack(__uint_as_float(sv[2 * i]), __uint_as_float(sv[2 * i + 1])), c2, nm2), a0, a1);
-              const uint64_t e2 = (i & 7) < POLY ? poly_exp2_x2(fminf(a0, 126.0f), fminf(a1, 126.0f))
+              const uint64_t e2 = (i & 7) < POLY ? poly_exp2_x2<OP>(fminf(a0, 126.0f), fminf(a1, 126.0f))
                                                  : f2_pack(fast_exp2(a0), fast_exp2(a1));
               rs2[i & 3] = f2_add(rs2[i & 3], e2);
               float e0, e1;
@@ -606,7 +606,8 @@ cudaError_t launch_attention_tc3(const CUtensorMap& tm_q, const CUtensorMap& tm_
 }
 
 // The operator runs the same kernel with two eighths of the exponentials on the FP32 pipe, the
-// encoder's measured best.
+// encoder's measured best, but by a polynomial that is exact to fp32: lse is a result here (16 x 1024 tokens of
+// 20 x 64 heads: 126 us, 122 with the encoder's 7.5e-5, 130 with all of them on the special-function unit).
 template <int DH, typename E>
 cudaError_t launch_op(const CUtensorMap& tm_q, const CUtensorMap& tm_kv, const AttnParams& p, int B, cudaStream_t s) {
   auto kernel = attention_tc3_kernel<DH, 2, 3, true, 0, E, true>;

@@ -1092,3 +1092,18 @@ def test_attention_backward_of_ragged_batches_is_reproducible(m, dh):
     check_backward(cu, qkv, 12, out, lse, dout, dqkv)
     for _ in range(3):
         assert torch.equal(run_backward(m, cu, qkv, 12, 500, out, lse, dout), dqkv)
+
+
+@pytest.mark.parametrize("dh", [16, 64])
+def test_attention_lse_is_exact_to_32_bits(m, dh):
+    """Exponentials within 2^-21 of exact (2.2e-7, or the exp2 instruction's 2^-22 with its rounding), summed in 32
+    bits: 32 of a row's columns at a time, then over the steps, and rescaled at most once a step."""
+    H, lens = 3, [1, 2, 3, 5, 33, 64, 200, 700]
+    cu, qkv, _ = attention_inputs(lens, H, dh, "bf16", seed=110 + dh, sharp=0.5)
+    out, lse = run_forward(m, cu, qkv, H, 700)
+    scale = dh ** -0.5
+    for a, b in sequences(cu):
+        q, k, _ = (split_heads(x, H) for x in qkv[a:b].split(H * dh, 1))
+        want = torch.logsumexp(scale * q @ k.transpose(-1, -2), -1)
+        es = score_error(q, k, scale).amax(-1)
+        within(lse[:, a:b], want, es + 2.0 ** -21 + (32 + 3 * (b - a) / 32) * E + 8 * E * (1 + want.abs()), "lse")
