@@ -64,6 +64,8 @@ struct QuadRow {
   }
 };
 
+// 90600 x 33 fp32, k = 5: 13 us, 16 on cold caches (24 MB: 0.9 and 0.75 TB/s). Bound by the instructions of
+// the top k, 66 % of the issue rate; a thread per row took 14 us, a warp per row 111.
 template <typename E, int N>
 __global__ void __launch_bounds__(128) logprobs_quad_kernel(const LogitsOp p) {
   const QuadRow r(p.T);
@@ -190,6 +192,7 @@ struct QuadTeacher {
   __device__ __forceinline__ float prob(int c) const { return id[c] >= 0 ? fast_exp2(v[c] * kLog2e) : 0.0f; }
 };
 
+// 65536 x 33 fp32, k up to 16: loss 7.6 us, gradient 10.4 (9.6 and 12.4 on cold caches); issue 52 and 58 %.
 template <typename E, int N, int K>
 __global__ void __launch_bounds__(128) distill_loss_quad_kernel(const LogitsOp p) {
   const QuadRow r(p.T);
@@ -451,6 +454,7 @@ __device__ void row_top(const LogitsOp& p, const E* x, int64_t t, float best, in
   }
 }
 
+// 512 x 32768 bf16: 23 us, 27 on cold caches (34 MB read once from HBM, the second pass from L2): issue 73 %.
 template <int NT, typename E>
 __global__ void __launch_bounds__(NT) logprobs_row_kernel(const LogitsOp p) {
   const int64_t t = blockIdx.x;
@@ -497,6 +501,8 @@ __device__ __forceinline__ bool teacher(const LogitsOp& p, int64_t t, int lane, 
   return m > -INFINITY;
 }
 
+// 1021 x 32003 fp16: loss 20 us, gradient 25 (22 and 27 on cold caches: 3.0 and 4.8 TB/s). The loss is bound by its
+// exponentials (special-function unit 53 %) and a row's latency, the gradient by the latter.
 template <int NT, typename E>
 __global__ void __launch_bounds__(NT) distill_loss_row_kernel(const LogitsOp p) {
   const int64_t t = blockIdx.x;
