@@ -357,25 +357,29 @@ __global__ void __launch_bounds__(kThreads3, 2)
           if (j == 0) mc = max32();
           float ls = exps();
           if (__any_sync(0xffffffffu, !(ls <= p.rescale_sum) && (!OP || q0 + t * kQ + r < len))) {
-            // j >= 1 here: with the exact max of tile 0 every P of step 0 is at most 1.
+            // At j = 0 mc is the exact max and every P is at most 1, unless a score is not finite or so large that
+            // rounding mc matters. There is no O yet then, and no PV(-1) to wait for: step[2t + 1] would only
+            // complete with a second key tile.
             load_s();
             const float m_new = fmaxf(mc, max32());
             const float alpha = fast_exp2(mc - m_new);
-            if (!mbar_wait_spin(&step[2 * t + ((j - 1) & 1)], (((j - 1) >> 1) + 1) & 1, p.err, kDevTimeoutEpilogue)) {
-              ok = false;
-              break;
-            }
-            tc_fence_after();
+            if (j > 0) {
+              if (!mbar_wait_spin(&step[2 * t + ((j - 1) & 1)], (((j - 1) >> 1) + 1) & 1, p.err, kDevTimeoutEpilogue)) {
+                ok = false;
+                break;
+              }
+              tc_fence_after();
 #pragma unroll 1
-            for (int oc = 0; oc < kD; oc += 16) {
-              uint32_t o[16];
-              tmem_ld16(t_o + oc, o);
-              tmem_ld_wait();
+              for (int oc = 0; oc < kD; oc += 16) {
+                uint32_t o[16];
+                tmem_ld16(t_o + oc, o);
+                tmem_ld_wait();
 #pragma unroll
-              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-              tmem_st16(t_o + oc, o);
+                for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                tmem_st16(t_o + oc, o);
+              }
+              tmem_st_wait();
             }
-            tmem_st_wait();
             l *= alpha;
             mc = m_new;
             ls = exps();
