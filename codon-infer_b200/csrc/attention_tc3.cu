@@ -334,7 +334,7 @@ __global__ void __launch_bounds__(kThreads3, 2)
             for (int u = 0; u < 8; ++u) pm[u] = fmaxf(pm[u], __uint_as_float(sv[u + 24]));
             return fmax3f(fmax3f(pm[0], pm[1], pm[2]), fmax3f(pm[3], pm[4], pm[5]), fmaxf(pm[6], pm[7])) * c;
           };
-          auto exps = [&]() {
+          auto exps = [&](auto poly) {  // that many eighths of them on the FP32 pipe
             const uint64_t c2 = f2_pack(c, c), nm2 = f2_pack(-mc, -mc);
             uint64_t rs2[4];
 #pragma unroll
@@ -343,8 +343,9 @@ __global__ void __launch_bounds__(kThreads3, 2)
             for (int i = 0; i < 16; ++i) {
               float a0, a1;
               f2_unpack(f2_fma(f2_pack(__uint_as_float(sv[2 * i]), __uint_as_float(sv[2 * i + 1])), c2, nm2), a0, a1);
-              const uint64_t e2 = (i & 7) < POLY ? poly_exp2_x2<OP>(fminf(a0, 126.0f), fminf(a1, 126.0f))
-                                                 : f2_pack(fast_exp2(a0), fast_exp2(a1));
+              const uint64_t e2 = (i & 7) < decltype(poly)::value
+                                      ? poly_exp2_x2<OP>(fminf(a0, 126.0f), fminf(a1, 126.0f))
+                                      : f2_pack(fast_exp2(a0), fast_exp2(a1));
               rs2[i & 3] = f2_add(rs2[i & 3], e2);
               float e0, e1;
               f2_unpack(e2, e0, e1);
@@ -355,7 +356,7 @@ __global__ void __launch_bounds__(kThreads3, 2)
             return r0 + r1;
           };
           if (j == 0) mc = max32();
-          float ls = exps();
+          float ls = exps(std::integral_constant<int, POLY>());
           if (__any_sync(0xffffffffu, !(ls <= p.rescale_sum) && (!OP || q0 + t * kQ + r < len))) {
             // At j = 0 mc is the exact max and every P is at most 1, unless a score is not finite or so large that
             // rounding mc matters. There is no O yet then, and no PV(-1) to wait for: step[2t + 1] would only
@@ -382,7 +383,9 @@ __global__ void __launch_bounds__(kThreads3, 2)
             }
             l *= alpha;
             mc = m_new;
-            ls = exps();
+            // A NaN score comes out of the FP32-pipe exponentials as 2^126, which trips the check. Taken again on
+            // the special-function unit it is a NaN in P and in l, as it has to be in a caller's result.
+            ls = exps(std::integral_constant<int, OP ? 0 : POLY>());
           }
           l += ls;
         } else {

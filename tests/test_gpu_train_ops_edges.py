@@ -45,6 +45,31 @@ def test_attention_bad_rows_of_short_sequences_are_written(m, kind, bad):
                 assert torch.equal(out2[at], out[at]) and torch.equal(lse2[:, at], lse[:, at])
 
 
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_attention_a_bad_key_shows_in_every_row(m, kind, bad):
+    """One key of one head is not finite, at every place of the first and of a later key tile: every query of that
+    sequence and head has a score that is NaN or +inf, so no distribution; other heads and sequences do not see it."""
+    H, dh = 3, 32
+    places = list(range(64)) + [0, 5, 19, 31]
+    lens = [96] * 64 + [32] * 4
+    cu, qkv, _ = ops.attention_inputs(lens, H, dh, kind, seed=210)
+    c, d = cu.tolist(), H * dh
+    qkv[:, dh:dh + 8] = qkv[:, dh:dh + 8].abs() + 0.5   # head 1's queries: an infinite key scores +inf
+    out, lse = ops.run_forward(m, cu, qkv, H, 96)
+    ops.check_forward(cu, qkv, H, out, lse)
+    qkv2 = qkv.clone()
+    for b, at in enumerate(places):
+        qkv2[c[b] + at, d + dh + b % 8] = bad
+    out2, lse2 = ops.run_forward(m, cu, qkv2, H, 96)
+    m.check_device()
+    head = slice(dh, 2 * dh)
+    rows = torch.isnan(out2[:, head]).all(1) & torch.isnan(lse2[1])
+    assert rows.all(), f"finite in {(~rows).sum().item()} rows, the first of sequence {int(rows.logical_not().nonzero()[0]) // 96}"
+    out2[:, head], lse2[1] = out[:, head], lse[1]
+    assert torch.equal(out2, out) and torch.equal(lse2, lse)
+
+
 @pytest.mark.parametrize("dim, heads", [(640, 10), (320, 20)])
 def test_encoder_forward_of_a_short_sequence_with_nan(esm, dim, heads):
     """The encoder's own attention: heads of 64 and of 16 columns, 1 to 33 tokens, one of them NaN."""
