@@ -58,6 +58,7 @@ struct Tc3 {
   static constexpr uint32_t kDescHi = DH == 64 ? kSw128DescHi : kSw64DescHi;
 };
 constexpr uint32_t kTmemCols3 = 256;
+constexpr float kRoundedMax = 4194304.0f;  // OP: running maxima below this (in the exp2 domain) are used rounded
 constexpr float kLog2e = 1.4426950408889634f;
 // The running max used for P is refreshed only when a row's max grows by more than 2^8 (in the
 // exp2 domain); until then P <= 256, exact in fp16's relative precision, and O and l share the
@@ -292,6 +293,7 @@ __global__ void __launch_bounds__(kThreads3, 2)
       const uint32_t t_o = tmem + lane_off + o_col<DH>(t);
       const float c = p.scale * kLog2e;
       float mc = -INFINITY;  // running max in the exp2 domain (max score * c)
+      float m_big = 0.0f;    // OP: the running max score itself where it is too large for mc, which is 0 then
       float l = 0.0f;
       bool ok = true;
       for (int j = 0; j < nkv && ok; ++j) {
@@ -332,9 +334,23 @@ __global__ void __launch_bounds__(kThreads3, 2)
               pm[u] = fmax3f(__uint_as_float(sv[u]), __uint_as_float(sv[u + 8]), __uint_as_float(sv[u + 16]));
 #pragma unroll
             for (int u = 0; u < 8; ++u) pm[u] = fmaxf(pm[u], __uint_as_float(sv[u + 24]));
-            return fmax3f(fmax3f(pm[0], pm[1], pm[2]), fmax3f(pm[3], pm[4], pm[5]), fmaxf(pm[6], pm[7])) * c;
+            return fmax3f(fmax3f(pm[0], pm[1], pm[2]), fmax3f(pm[3], pm[4], pm[5]), fmaxf(pm[6], pm[7]));
           };
-          auto exps = [&](auto poly) {  // that many eighths of them on the FP32 pipe
+          // OP: P = 2^(S c - mc) while mc, the rounded product, is below 2^22. Its rounding, at most 2^-3, is the
+          // same for every key of the row and cancels. Above, it could take all P of a row out of fp16's range, so
+          // P = 2^((S - m_big) c) in every step of such a row, by way of the check below.
+          auto set_max = [&](float top) {
+            mc = top * c;
+            m_big = 0.0f;
+            if (!(fabsf(mc) < kRoundedMax)) {
+              m_big = top;
+              mc = 0.0f;
+            }
+          };
+          auto exps = [&](auto again) {
+            constexpr bool kExact = OP && decltype(again)::value;
+            constexpr int kPoly = kExact ? 0 : POLY;
+            const uint64_t mb2 = f2_pack(m_big, m_big);
             const uint64_t c2 = f2_pack(c, c), nm2 = f2_pack(-mc, -mc);
             uint64_t rs2[4];
 #pragma unroll
@@ -342,8 +358,10 @@ __global__ void __launch_bounds__(kThreads3, 2)
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
               float a0, a1;
-              f2_unpack(f2_fma(f2_pack(__uint_as_float(sv[2 * i]), __uint_as_float(sv[2 * i + 1])), c2, nm2), a0, a1);
-              const uint64_t e2 = (i & 7) < decltype(poly)::value
+              uint64_t s2 = f2_pack(__uint_as_float(sv[2 * i]), __uint_as_float(sv[2 * i + 1]));
+              if constexpr (kExact) s2 = f2_sub(s2, mb2);
+              f2_unpack(f2_fma(s2, c2, nm2), a0, a1);
+              const uint64_t e2 = (i & 7) < kPoly
                                       ? poly_exp2_x2<OP>(fminf(a0, 126.0f), fminf(a1, 126.0f))
                                       : f2_pack(fast_exp2(a0), fast_exp2(a1));
               rs2[i & 3] = f2_add(rs2[i & 3], e2);
@@ -355,15 +373,25 @@ __global__ void __launch_bounds__(kThreads3, 2)
             f2_unpack(f2_add(f2_add(rs2[0], rs2[1]), f2_add(rs2[2], rs2[3])), r0, r1);
             return r0 + r1;
           };
-          if (j == 0) mc = max32();
-          float ls = exps(std::integral_constant<int, POLY>());
-          if (__any_sync(0xffffffffu, !(ls <= p.rescale_sum) && (!OP || q0 + t * kQ + r < len))) {
-            // At j = 0 mc is the exact max and every P is at most 1, unless a score is not finite or so large that
-            // rounding mc matters. There is no O yet then, and no PV(-1) to wait for: step[2t + 1] would only
-            // complete with a second key tile.
+          if (j == 0) {
+            if constexpr (OP) set_max(max32());
+            else mc = max32() * c;
+          }
+          float ls = exps(std::false_type());
+          if (__any_sync(0xffffffffu, OP ? (!(ls <= p.rescale_sum) || m_big != 0.0f) && q0 + t * kQ + r < len
+                                         : !(ls <= p.rescale_sum))) {
+            // At j = 0 mc is the exact max and every P is at most 1, unless a score is not finite or very large.
+            // There is no O yet then, and no PV(-1) to wait for: step[2t + 1] would only complete with a second
+            // key tile.
             load_s();
-            const float m_new = fmaxf(mc, max32());
-            const float alpha = fast_exp2(mc - m_new);
+            const float top = max32(), mc_old = mc, m_big_old = m_big;
+            if constexpr (OP) {
+              if (m_big != 0.0f) set_max(fmaxf(m_big, top));
+              else if (top * c > mc) set_max(top);
+            } else {
+              mc = fmaxf(mc, top * c);
+            }
+            const float alpha = fast_exp2(OP ? fmaf(m_big_old - m_big, c, mc_old - mc) : mc_old - mc);
             if (j > 0) {
               if (!mbar_wait_spin(&step[2 * t + ((j - 1) & 1)], (((j - 1) >> 1) + 1) & 1, p.err, kDevTimeoutEpilogue)) {
                 ok = false;
@@ -382,10 +410,9 @@ __global__ void __launch_bounds__(kThreads3, 2)
               tmem_st_wait();
             }
             l *= alpha;
-            mc = m_new;
-            // A NaN score comes out of the FP32-pipe exponentials as 2^126, which trips the check. Taken again on
+            // OP: a NaN score comes out of the FP32-pipe exponentials as 2^126, which trips the check. Taken again on
             // the special-function unit it is a NaN in P and in l, as it has to be in a caller's result.
-            ls = exps(std::integral_constant<int, OP ? 0 : POLY>());
+            ls = exps(std::true_type());
           }
           l += ls;
         } else {
@@ -538,7 +565,7 @@ __global__ void __launch_bounds__(kThreads3, 2)
             }
           }
         }
-        if (row < len && p.lse) p.lse[static_cast<size_t>(h) * p.T + start + row] = (mc + log2f(l)) / kLog2e;
+        if (row < len && p.lse) p.lse[static_cast<size_t>(h) * p.T + start + row] = ((OP ? fmaf(m_big, c, mc) : mc) + log2f(l)) / kLog2e;
       }
     }
   }

@@ -70,6 +70,61 @@ def test_attention_a_bad_key_shows_in_every_row(m, kind, bad):
     assert torch.equal(out2, out) and torch.equal(lse2, lse)
 
 
+def check_exact_scores(cu, qkv, H, out, lse, scale):
+    """Where every score is a multiple of its last bit in fp32, the products are exact, and exponentials take the
+    difference to the maximum, which is exact too: the probabilities are as good as those of small scores."""
+    U, d = ops.half_step(qkv.dtype), qkv.shape[1] // 3
+    for a, b in ops.sequences(cu):
+        q, k, v = (ops.split_heads(x, H) for x in qkv[a:b].split(d, 1))
+        s = scale * q @ k.transpose(-1, -2)
+        assert torch.equal((s / scale).float().double() * scale, s)
+        want_lse = torch.logsumexp(s, -1)
+        p = torch.softmax(s, -1)
+        # Exponentials and their arguments (down to e^-40; below, they are less than U of nothing), sums of b - a terms.
+        rel = 2.0 ** -20 + 40 * 4 * ops.E + (b - a) * ops.E
+        want = p @ v
+        ops.within(ops.split_heads(out[a:b], H), want, (U + rel) * (p @ v.abs()) + U * want.abs() + 2.0 ** -25, "out")
+        ops.within(lse[:, a:b], want_lse, 8 * ops.E * want_lse.abs() + rel, "lse")
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("terms, step", [(1, 2.0 ** -7), (2, 2.0 ** 6), (8, 2.0 ** 8), (32, 2.0 ** 10)])
+def test_attention_large_scores(m, kind, sign, terms, step):
+    """Scores whose maximum is 2^19 to 2^31, where its product with log2 e rounds by up to 128, and whose
+    differences are a few bits of that, beside rows with ordinary scores."""
+    dh, lens = 64, [1, 20, 33, 150]
+    T = sum(lens)
+    cu, qkv, _ = ops.attention_inputs(lens, 1, dh, kind, seed=220)
+    q, k = qkv[:, :dh], qkv[:, dh:2 * dh]
+    q.zero_(), k.zero_()
+    big = 2.0 ** 7 if terms == 1 else 2.0 ** 14
+    q[:, :terms] = sign * big
+    k[:, :terms] = big
+    at = torch.arange(T, device="cuda")
+    q[:, 40] = step                                  # S = sign * terms * big^2 + step * (0 .. 7)
+    k[:, 40] = ((at * 5) % 8).to(k.dtype)
+    q[3::7, :terms] = 0.0                            # ordinary rows in the same warps
+    for scale in (0.25 / step, 1.0 / step, 16.0 / step, 256.0 / step):
+        out, lse = ops.run_forward(m, cu, qkv, 1, 150, scale=scale)
+        m.check_device()
+        check_exact_scores(cu, qkv, 1, out, lse, scale)
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+def test_attention_maximum_grows_through_large_scores(m, kind):
+    """Key tiles whose scores rise from -2^24 through ordinary ones to 2^24 (log2), and fall again."""
+    dh, L = 32, 300
+    cu, qkv, _ = ops.attention_inputs([L], 1, dh, kind, seed=221)
+    q, k = qkv[:, :dh], qkv[:, dh:2 * dh]
+    q.zero_(), k.zero_()
+    steps = [-2.0 ** 12, -2.0 ** 9, -8.0, -1.0, 0.0, 1.0, 2.0 ** 9, 2.0 ** 12, 2.0 ** 12, 2.0 ** 9]
+    k[:, 0] = torch.tensor(steps, device="cuda").repeat_interleave(32)[:L].to(k.dtype)
+    q[0::3, 0], q[1::3, 0], q[2::3, 0] = 2.0 ** 12, -2.0 ** 12, 1.0
+    out, lse = ops.run_forward(m, cu, qkv, 1, L, scale=1.0)
+    check_exact_scores(cu, qkv, 1, out, lse, 1.0)
+
+
 @pytest.mark.parametrize("dim, heads", [(640, 10), (320, 20)])
 def test_encoder_forward_of_a_short_sequence_with_nan(esm, dim, heads):
     """The encoder's own attention: heads of 64 and of 16 columns, 1 to 33 tokens, one of them NaN."""
