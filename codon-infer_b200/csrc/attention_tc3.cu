@@ -58,7 +58,8 @@ struct Tc3 {
   static constexpr uint32_t kDescHi = DH == 64 ? kSw128DescHi : kSw64DescHi;
 };
 constexpr uint32_t kTmemCols3 = 256;
-constexpr float kRoundedMax = 4194304.0f;  // OP: running maxima below this (in the exp2 domain) are used rounded
+// OP: running maxima below this (in the exp2 domain) are used rounded; and the maximum of scores that are all -inf.
+constexpr float kRoundedMax = 4194304.0f, kNoScore = -1e30f;
 constexpr float kLog2e = 1.4426950408889634f;
 // The running max used for P is refreshed only when a row's max grows by more than 2^8 (in the
 // exp2 domain); until then P <= 256, exact in fp16's relative precision, and O and l share the
@@ -338,8 +339,10 @@ __global__ void __launch_bounds__(kThreads3, 2)
           };
           // OP: P = 2^(S c - mc) while mc, the rounded product, is below 2^22. Its rounding, at most 2^-3, is the
           // same for every key of the row and cancels. Above, it could take all P of a row out of fp16's range, so
-          // P = 2^((S - m_big) c) in every step of such a row, by way of the check below.
+          // P = 2^((S - m_big) c) in every step of such a row, by way of the check below. Scores that are all -inf so
+          // far get a finite maximum, from which a later score can take over.
           auto set_max = [&](float top) {
+            top = fmaxf(top, kNoScore);
             mc = top * c;
             m_big = 0.0f;
             if (!(fabsf(mc) < kRoundedMax)) {

@@ -276,8 +276,9 @@ enum { ESM_F32 = 0, ESM_F16 = 1, ESM_BF16 = 2 };
  * rows of the buffers: rows behind the last sequence are left as they are. head_dim is a multiple of 8
  * up to 64, scale in [1e-6, 1e6]; B and n_heads are at most 65535, T at most 2^30. d_lse [H, T] or NULL (the
  * backward pass needs it). Scores, sums and outputs are accumulated in fp32, probabilities are rounded to
- * `type` for the product with V. Offsets that do not fit (descending, beyond T or longer than
- * max_len) are noticed on the device: that sequence, and in the backward pass perhaps others, is skipped and
+ * `type` for the product with V. A row with a score that is NaN or +inf has NaN in out and lse; scores of -inf have
+ * probability 0, and a row with no other has NaN in out and lse -inf; finite q k are at most 1e30 in
+ * magnitude. Offsets that do not fit (descending, beyond T or longer than max_len) are noticed on the device: that sequence, and in the backward pass perhaps others, is skipped and
  * esm_check_device returns ESM_EINVAL. */
 int esm_attention(esm_ctx* ctx, int32_t type, const void* d_qkv, int64_t ld_qkv, const int32_t* d_cu_seqlens,
                   int32_t B, int32_t T, int32_t max_len, int32_t n_heads, int32_t head_dim, float scale, void* d_out,

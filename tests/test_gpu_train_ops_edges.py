@@ -125,6 +125,35 @@ def test_attention_maximum_grows_through_large_scores(m, kind):
     check_exact_scores(cu, qkv, 1, out, lse, 1.0)
 
 
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("ruled_out", [1, 31, 32, 33, 64, 99])
+def test_attention_scores_of_minus_infinity(m, kind, ruled_out):
+    """Keys whose scores are -inf have no part in the result, also when they fill the first key tiles; a row that has
+    nothing else has no distribution."""
+    H, dh, L = 2, 24, 100
+    cu, qkv, _ = ops.attention_inputs([L, 40, L], H, dh, kind, seed=222)
+    d = H * dh
+    qkv[:, :d] = qkv[:, :d].abs() + 0.25
+    rest = qkv.clone()
+    qkv[:ruled_out, d + 3] = -math.inf               # head 0 of the first sequence
+    qkv[L + 40:, d + dh:2 * d] = -math.inf           # head 1 of the last one, every key
+    out, lse = ops.run_forward(m, cu, qkv, H, L)
+    m.check_device()
+    other, other_lse = ops.run_forward(m, cu, rest, H, L)
+    assert torch.isnan(out[L + 40:, dh:]).all() and (lse[1, L + 40:] == -math.inf).all()
+    q, k, v = (x[:, 0] for x in rest[:L].double().unflatten(1, (3, H, dh)).unbind(1))
+    s = dh ** -0.5 * q @ k[ruled_out:].t()
+    p = torch.softmax(s, 1)
+    es = ops.score_error(q, k, dh ** -0.5).amax()
+    want = p @ v[ruled_out:]
+    rel = ops.half_step(qkv.dtype) + 2 * es + 2.0 ** -19
+    ops.within(out[:L, :dh], want, rel * (p @ v[ruled_out:].abs()) + ops.half_step(qkv.dtype) * want.abs() + 2.0 ** -25, "out")
+    ops.within(lse[0, :L], torch.logsumexp(s, 1), es + 2.0 ** -19 + 8 * ops.E * s.abs().amax(1), "lse")
+    out[:L, :dh], lse[0, :L] = other[:L, :dh], other_lse[0, :L]
+    out[L + 40:, dh:], lse[1, L + 40:] = other[L + 40:, dh:], other_lse[1, L + 40:]
+    assert torch.equal(out, other) and torch.equal(lse, other_lse)
+
+
 @pytest.mark.parametrize("dim, heads", [(640, 10), (320, 20)])
 def test_encoder_forward_of_a_short_sequence_with_nan(esm, dim, heads):
     """The encoder's own attention: heads of 64 and of 16 columns, 1 to 33 tokens, one of them NaN."""
