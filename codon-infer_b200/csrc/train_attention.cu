@@ -32,8 +32,8 @@
 // In key items lse and D belong to the columns of a thread's row. Reading them for every row costs more
 // shared-memory bandwidth than all operand reads of the tensor cores (a 16-byte broadcast read is four
 // wavefronts), so they are subtracted by the tensor cores: one more K step of 16 with constants in every row of
-// A, (2^15, 1, 2^-10) for fp16 and ones for bf16, and -lse / scale, or -D, split into three parts of the
-// operand type in B. For fp16 that covers magnitudes up to 2^30, to 2^-33 or 2^-24 relative.
+// A, (2^15, 2^3, 2^-9) for fp16 and ones for bf16, and -lse / scale, or -D, split into three parts of the
+// operand type in B. For fp16 that covers magnitudes up to 2^30, to 2^-34 or 2^-24 relative.
 //
 // Heads narrower than 32 or 64 columns arrive zero-padded by the 3-D tensor maps. Rows past the
 // sequence's end in the last streamed tile are cleared in shared memory (they belong to other
@@ -191,15 +191,17 @@ __device__ __forceinline__ int ds_exponent(const BwdParams& p, int start, int le
   return min(60, max(-60, 13 - ilogbf(bound)));
 }
 
-// x as three values of E, times 2^15, 1 and 2^-10 for fp16 (whose range the factors extend) and 1
-// for bf16, packed into the first 16 bytes of a K step (the other elements are zero).
+// x as three values of E, times 2^15, 2^3 and 2^-9 for fp16 (whose range the factors extend) and 1
+// for bf16, packed into the first 16 bytes of a K step (the other elements are zero). fp16: for |x| <= 2^30 the
+// first part is at most 2^15 and leaves at most 2^18, the second is at most 2^15 and leaves at most 2^6, the
+// third is at most 2^15; what it leaves is half of its last bit, 2^-34 where that is subnormal.
 template <typename E>
 __device__ __forceinline__ uint4 split_parts(float x) {
   if constexpr (std::is_same<E, __half>::value) {
     const __half h0 = __float2half_rn(x * (1.0f / 32768.0f));
     float r = fmaf(-32768.0f, __half2float(h0), x);
-    const __half h1 = __float2half_rn(fminf(fmaxf(r, -65504.0f), 65504.0f));
-    r = (r - __half2float(h1)) * 1024.0f;
+    const __half h1 = __float2half_rn(r * 0.125f);
+    r = fmaf(-8.0f, __half2float(h1), r) * 512.0f;
     const __half2 h01 = __halves2half2(h0, h1);
     return make_uint4(*reinterpret_cast<const uint32_t*>(&h01), pack2<E>(r, 0.0f), 0u, 0u);
   } else {  // by truncation: each part is the upper half of what is left
@@ -212,7 +214,7 @@ __device__ __forceinline__ uint4 split_parts(float x) {
 }
 template <typename E>
 __device__ __forceinline__ uint4 split_factors() {
-  if constexpr (std::is_same<E, __half>::value) return make_uint4(pack2<E>(32768.0f, 1.0f), pack2<E>(1.0f / 1024.0f, 0.0f), 0u, 0u);
+  if constexpr (std::is_same<E, __half>::value) return make_uint4(pack2<E>(32768.0f, 8.0f), pack2<E>(1.0f / 512.0f, 0.0f), 0u, 0u);
   else return make_uint4(pack2<E>(1.0f, 1.0f), pack2<E>(1.0f, 0.0f), 0u, 0u);
 }
 
@@ -542,8 +544,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           uint4 part_l[2], part_d[2];
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
-            // P = exp2(c (S - lse / scale)), times 2^kProbExp; 0 past the end.
-            const float x = lane + 32 * u < kept ? -(next_l[u] - kProbExp * 0.69314718f) * inv_scale : (kScaled ? -1.9e9f : -1e30f);
+            // P = exp2(c (S - lse / scale)), times 2^kProbExp; 0 past the end, where S is 0 and the first part
+            // alone is the constant.
+            const float x = lane + 32 * u < kept ? -(next_l[u] - kProbExp * 0.69314718f) * inv_scale : (kScaled ? -57344.0f * 32768.0f : -1e30f);
             part_l[u] = split_parts<E>(x);
             part_d[u] = split_parts<E>(-next_d[u]);
           }

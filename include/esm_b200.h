@@ -291,7 +291,7 @@ int esm_attention(esm_ctx* ctx, int32_t type, const void* d_qkv, int64_t ld_qkv,
  *   dS = P (dout V^T - D),  dQ = scale dS K,  dK = scale dS^T Q.
  * P and dS are rounded to `type` for the products; with ESM_F16 each is scaled by a power of two
  * first (from the largest |dout| and |V| of the sequence and head), so small gradients do not
- * underflow; products q k and sums of dout out beyond 2^30 in magnitude are outside its range.
+ * underflow; its range is |lse| / scale and sums of dout out up to 1e9.
  * d_workspace: esm_attention_backward_workspace bytes, 16-byte aligned. */
 int esm_attention_backward_workspace(int32_t B, int32_t T, int32_t n_heads, size_t* bytes);
 int esm_attention_backward(esm_ctx* ctx, int32_t type, const void* d_qkv, int64_t ld_qkv,

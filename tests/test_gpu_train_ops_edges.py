@@ -154,6 +154,44 @@ def test_attention_scores_of_minus_infinity(m, kind, ruled_out):
     assert torch.equal(out, other) and torch.equal(lse, other_lse)
 
 
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("n", range(20, 30))
+def test_attention_backward_of_large_scores(m, kind, n):
+    """lse / scale of every query spread over [2^n, 2^(n+1)) up to 1e9: it reaches the key items in parts of 16 bits."""
+    dh, lens, scale = 64, [200, 33], 2.0 ** -19
+    T = sum(lens)
+    cu, qkv, dout = ops.attention_inputs(lens, 1, dh, kind, seed=230 + n)
+    q, k = qkv[:, :dh], qkv[:, dh:2 * dh]
+    q.zero_(), k.zero_()
+    top = 2.0 ** 16 if n < 29 else 1.8 * 2.0 ** 15
+    at = torch.arange(T, device="cuda")
+    q[:, 0] = (2.0 ** 15 + (top - 2.0 ** 15) * ((at * 0.6180339887) % 1.0)).clamp(max=65000).to(q.dtype)
+    q[:, 1] = (at * 37 % 256 * 8).to(q.dtype)
+    q[:, 2] = 16.0
+    k[:, 0], k[:, 1] = 2.0 ** (n - 15), 2.0 ** (n - 21)
+    k[:, 2] = (12000 * ops.randn(231, T)).to(k.dtype)       # scores that differ by about 0.4
+    out, lse = ops.run_forward(m, cu, qkv, 1, 200, scale=scale)
+    ops.check_forward(cu, qkv, 1, out, lse, scale)
+    dqkv = ops.run_backward(m, cu, qkv, 1, 200, out, lse, dout, scale=scale)
+    ops.check_backward(cu, qkv, 1, out, lse, dout, dqkv, scale)
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("terms", [1, 2, 3])
+def test_attention_backward_of_large_sums(m, kind, terms):
+    """Sums of dout out up to 1e9, beside which the rest of dS is small."""
+    dh, lens = 64, [150, 40]
+    T = sum(lens)
+    cu, qkv, dout = ops.attention_inputs(lens, 1, dh, kind, seed=240)
+    v = qkv[:, 2 * dh:]
+    v[:, :terms] = 2.0 ** 15
+    dout[:, :terms] = (2.0 ** 13 * (0.51 + 0.48 * torch.rand(T, 1, device="cuda", generator=torch.Generator(device="cuda").manual_seed(241)))).to(dout.dtype)
+    dout[:, 10:] *= 2.0 ** 12
+    out, lse = ops.run_forward(m, cu, qkv, 1, 150)
+    dqkv = ops.run_backward(m, cu, qkv, 1, 150, out, lse, dout)
+    ops.check_backward(cu, qkv, 1, out, lse, dout, dqkv)
+
+
 @pytest.mark.parametrize("dim, heads", [(640, 10), (320, 20)])
 def test_encoder_forward_of_a_short_sequence_with_nan(esm, dim, heads):
     """The encoder's own attention: heads of 64 and of 16 columns, 1 to 33 tokens, one of them NaN."""
