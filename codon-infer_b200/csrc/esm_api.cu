@@ -52,7 +52,7 @@ struct esm_ctx {
   int contact_tc = 1;  // tcgen05 contact accumulation for head_dim 64 (ESM_CONTACT_TC=0: mma.sync kernel)
   std::mutex mu;
   std::string err;
-  int* d_err = nullptr;
+  int* d_err = nullptr;     // error words: of the encoder's calls, of the operators', and room for a copy of that
 
   // ---- weights ----
   bool loaded = false;
@@ -845,12 +845,17 @@ int forward_impl(esm_ctx* c, const int32_t* d_tokens, const int32_t* h_cu, int B
   return ESM_OK;
 }
 
-int check_device_word(esm_ctx* c) {
+// The errors of `op_word`, taken by the caller, and of the encoder's word. The operators have a word of their own
+// because they run on callers' streams: an encoder call would report theirs as its own otherwise.
+int check_device_word(esm_ctx* c, int op_word = 0) {
   int h = 0;
   ESM_CUDA(cudaMemcpy(&h, c->d_err, sizeof(int), cudaMemcpyDeviceToHost));
   if (h != 0) {
     cudaMemsetAsync(c->d_err, 0, sizeof(int), c->stream);
     cudaStreamSynchronize(c->stream);
+  }
+  h |= op_word;
+  if (h != 0) {
     if (h == esm::kDevBadToken)
       return fail(c, ESM_EINVAL, "a token id is outside [0, " + std::to_string(c->cfg.vocab_size) + ")");
     if (h == esm::kDevBadSeqlens)
@@ -976,8 +981,8 @@ int esm_ctx_create(int32_t device, esm_ctx** out) {
     events_ok = cudaEventCreateWithFlags(&c->ev_deq[b], cudaEventDisableTiming) == cudaSuccess &&
                 cudaEventCreateWithFlags(&c->ev_read[b], cudaEventDisableTiming) == cudaSuccess;
   if (!events_ok || cudaStreamCreateWithFlags(&c->stream, cudaStreamNonBlocking) != cudaSuccess ||
-      cudaMalloc(&c->d_err, sizeof(int)) != cudaSuccess ||
-      cudaMemsetAsync(c->d_err, 0, sizeof(int), c->stream) != cudaSuccess ||
+      cudaMalloc(&c->d_err, 3 * sizeof(int)) != cudaSuccess ||
+      cudaMemsetAsync(c->d_err, 0, 3 * sizeof(int), c->stream) != cudaSuccess ||
       cudaStreamSynchronize(c->stream) != cudaSuccess) {
     if (c->d_err) cudaFree(c->d_err);
     for (cudaStream_t st : {c->stream, c->side})
@@ -1781,7 +1786,12 @@ int esm_check_device(esm_ctx* c) {
   std::lock_guard<std::mutex> lk(c->mu);
   ESM_CUDA(cudaSetDevice(c->device));
   ESM_CUDA(cudaStreamSynchronize(c->stream));
-  return check_device_word(c);
+  // An operator may be running on another stream: its word is exchanged, not read and then cleared. On the legacy
+  // stream, so that operators on it, or on streams that synchronise with it, are seen.
+  int op_word = 0;
+  ESM_CUDA(esm::launch_take_word(c->d_err + 1, c->d_err + 2, nullptr));
+  ESM_CUDA(cudaMemcpy(&op_word, c->d_err + 2, sizeof(int), cudaMemcpyDeviceToHost));
+  return check_device_word(c, op_word);
 }
 
 /* ---- operators on device memory ---------------------------------------------------------------- */
@@ -1920,7 +1930,7 @@ int esm_attention(esm_ctx* c, int32_t type, const void* d_qkv, int64_t ld_qkv, c
   p.out = d_out;
   p.ld_out = ld_out;
   p.lse = d_lse;
-  p.err = c->d_err;
+  p.err = c->d_err + 1;
   ESM_CUDA(esm::launch_attention_op(p, s));
   return ESM_OK;
 }
@@ -1976,7 +1986,7 @@ int esm_attention_backward(esm_ctx* c, int32_t type, const void* d_qkv, int64_t 
   p.ld_dqkv = ld_dqkv;
   p.workspace = static_cast<float*>(d_workspace);
   p.num_sms = c->num_sms;
-  p.err = c->d_err;
+  p.err = c->d_err + 1;
   ESM_CUDA(esm::launch_attention_backward(p, s));
   return ESM_OK;
 }

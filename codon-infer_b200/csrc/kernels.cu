@@ -553,6 +553,8 @@ __global__ void dms_score_kernel(const float* __restrict__ logits, int V, const 
   }
 }
 
+__global__ void take_word_kernel(int* word, int* copy) { *copy = atomicExch(word, 0); }
+
 __global__ void wait_probe_kernel(int* err, uint64_t limit_ns) {
   __shared__ uint64_t bar;
   mbar_init(&bar, 1);
@@ -677,6 +679,11 @@ cudaError_t launch_dms_score(const float* logits, int V, const int32_t* tok_row,
 
 cudaError_t launch_wait_probe(int* err, uint64_t limit_ns, cudaStream_t s) {
   wait_probe_kernel<<<1, 1, 0, s>>>(err, limit_ns);
+  return cudaGetLastError();
+}
+
+cudaError_t launch_take_word(int* word, int* copy, cudaStream_t s) {
+  take_word_kernel<<<1, 1, 0, s>>>(word, copy);
   return cudaGetLastError();
 }
 

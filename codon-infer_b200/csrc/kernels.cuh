@@ -72,6 +72,8 @@ cudaError_t launch_dms_score(const float* logits, int V, const int32_t* tok_row,
 // One thread waits, with the kernels' bounded mbarrier wait and a limit of `limit_ns`, on a phase
 // that nothing completes; on timeout it records kDevTimeoutProbe in *err and returns.
 cudaError_t launch_wait_probe(int* err, uint64_t limit_ns, cudaStream_t s);
+// *copy = *word and *word = 0, as one exchange.
+cudaError_t launch_take_word(int* word, int* copy, cudaStream_t s);
 
 // ---- attention ------------------------------------------------------------------------------
 struct AttnParams {

@@ -260,7 +260,9 @@ int esm_matmul_tiled_noalloc(int32_t dtype, const float* d_x, const void* d_w, c
  * or host pointer, or a buffer that is written and overlaps another one, is ESM_EINVAL; a workspace
  * that is too small is ESM_ECAPACITY. A workspace holds nothing between calls; calls that may run
  * at the same time (two streams, two captured graphs) need one each. Results do not depend on how
- * often or beside what a call runs: sums are taken in a fixed order. Calls with no rows do nothing
+ * often or beside what a call runs: sums are taken in a fixed order. What an operator finds wrong on the device is
+ * reported by esm_check_device alone. A graph that holds calls is not replayed after its context is destroyed.
+ * Calls with no rows do nothing
  * (esm_layernorm_backward then writes zero weight gradients). */
 
 /* Element types of the operators' matrices (not the ESM_DTYPE_* storage types of weights). */
@@ -428,7 +430,10 @@ int esm_profile_read(esm_ctx* ctx, int32_t kind, double* total_ms, int64_t* laun
  * context is usable again. No trap, fault or unbounded loop is involved. */
 int esm_probe_wait_timeout(esm_ctx* ctx, int32_t limit_ms);
 
-/* Device error word check: ESM_ETIMEOUT if a kernel's bounded wait gave up since the last call. */
+/* Device errors since the last call: ESM_ETIMEOUT if a kernel's bounded wait gave up, ESM_EINVAL if a kernel
+ * found a bad argument. Encoder calls that wait report their own when they return; those of the operators on device
+ * memory are only reported here. Waits for the context's own stream and the legacy default stream: synchronise
+ * any other stream of an operator first, or its errors may be reported by a later call. */
 int esm_check_device(esm_ctx* ctx);
 
 #ifdef __cplusplus

@@ -209,3 +209,46 @@ def test_encoder_forward_of_a_short_sequence_with_nan(esm, dim, heads):
         assert not np.isfinite(logits[0, n - 1]).any()
     model.check_device()
     model.close()
+
+
+# ---- errors that are found on the device --------------------------------------------------------------
+
+@pytest.fixture
+def encoder(esm):
+    cfg = esm.EsmConfig(320, 1280, 1, 20, 33, 64, 0)
+    model = esm.Model(0)
+    model.load_tensors(cfg, esm.DTYPE_FP32, esm.synth_fp32_tensors(cfg, seed=3))
+    model.reserve(100, 4, 64)
+    yield model
+    model.close()
+
+
+def bad_offsets(model):
+    _, qkv, _ = ops.attention_inputs([64], 2, 16, "f16", seed=14)
+    ops.run_forward(model, torch.tensor([0, 40, 30, 64], dtype=torch.int32, device="cuda"), qkv, 2, 45)
+
+
+def test_an_operators_error_is_not_the_encoders(esm, encoder):
+    """Bad offsets of an operator do not fail the context's encoder calls, which leave them to check_device."""
+    seqs = [np.arange(n, dtype=np.int32) % 20 + 4 for n in (30, 12)]
+    logits, scores = encoder.forward(seqs)["logits"], encoder.score(seqs)["logp"]
+    bad_offsets(encoder)
+    torch.cuda.synchronize()
+    assert np.array_equal(encoder.forward(seqs)["logits"], logits)
+    assert np.array_equal(encoder.score(seqs)["logp"], scores)
+    with pytest.raises(esm.EsmError, match="token id"):
+        encoder.forward([np.full(5, 77, dtype=np.int32)])
+    with pytest.raises(esm.EsmError, match="cu_seqlens") as e:
+        encoder.check_device()
+    assert e.value.code == esm.ESM_EINVAL
+    encoder.check_device()
+
+
+def test_errors_on_another_stream_are_reported(esm, encoder):
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        bad_offsets(encoder)
+    s.synchronize()
+    with pytest.raises(esm.EsmError, match="cu_seqlens"):
+        encoder.check_device()
+    encoder.check_device()
