@@ -855,14 +855,15 @@ int check_device_word(esm_ctx* c, int op_word = 0) {
     cudaStreamSynchronize(c->stream);
   }
   h |= op_word;
-  if (h != 0) {
-    if (h == esm::kDevBadToken)
-      return fail(c, ESM_EINVAL, "a token id is outside [0, " + std::to_string(c->cfg.vocab_size) + ")");
-    if (h == esm::kDevBadSeqlens)
-      return fail(c, ESM_EINVAL, "cu_seqlens are not ascending offsets of sequences of at most max_len rows");
-    return fail(c, ESM_ETIMEOUT, "a device-side bounded wait gave up (code " + std::to_string(h) + ")");
-  }
-  return ESM_OK;
+  if (h == 0) return ESM_OK;
+  // Several calls may have left their bits since the last check: all are named, and a wait that gave up decides.
+  constexpr int kArguments = esm::kDevBadToken | esm::kDevBadSeqlens;
+  std::string what;
+  auto say = [&](const std::string& x) { what += (what.empty() ? "" : "; ") + x; };
+  if (h & ~kArguments) say("a device-side bounded wait gave up (code " + std::to_string(h & ~kArguments) + ")");
+  if (h & esm::kDevBadToken) say("a token id is outside [0, " + std::to_string(c->cfg.vocab_size) + ")");
+  if (h & esm::kDevBadSeqlens) say("cu_seqlens are not ascending offsets of sequences of at most max_len rows");
+  return fail(c, h & ~kArguments ? ESM_ETIMEOUT : ESM_EINVAL, what);
 }
 
 int validate_call(esm_ctx* c, const int32_t* h_cu, int B, bool contacts) {

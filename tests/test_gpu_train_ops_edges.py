@@ -252,3 +252,21 @@ def test_errors_on_another_stream_are_reported(esm, encoder):
     with pytest.raises(esm.EsmError, match="cu_seqlens"):
         encoder.check_device()
     encoder.check_device()
+
+
+def test_errors_of_several_calls_are_all_named(esm, encoder):
+    """Error bits are gathered until they are read: two bad arguments are not a wait that gave up."""
+    cu = np.array([0, 5], dtype=np.int32)
+    bad, logits = torch.full((5,), 77, dtype=torch.int32, device="cuda"), torch.empty(5, 33, device="cuda")
+    for _ in range(2):
+        encoder.forward_device(bad, cu, logits)
+        bad_offsets(encoder)
+        with pytest.raises(esm.EsmError, match="token id.*cu_seqlens") as e:
+            encoder.check_device()
+        assert e.value.code == esm.ESM_EINVAL
+    encoder.check_device()
+    encoder.forward_device(bad, cu, logits)
+    assert encoder.probe_wait_timeout(20) == esm.ESM_ETIMEOUT
+    message = esm.lib().esm_last_error(encoder._ctx).decode()
+    assert "wait gave up" in message and "token id" in message
+    encoder.check_device()
