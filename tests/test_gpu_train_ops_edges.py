@@ -211,6 +211,65 @@ def test_encoder_forward_of_a_short_sequence_with_nan(esm, dim, heads):
     model.close()
 
 
+# ---- distillation: temperatures and large logits --------------------------------------------------------
+
+def check_soft(x, ids, top, dloss, tau, loss, lse, dx):
+    """check_distill with bounds that do not grow with |x| / tau: exponents are differences to the row's maximum,
+    each with a relative error of 4 E, and 2^-21 in the exponential; lse and the loss are rounded once more."""
+    V = x.shape[1]
+    U = ops.half_step(x.dtype)
+    want, want_lse, q, p, any_, _, _ = ops.distill_64(x, ids, top, tau)
+    sums = (V / 32 + 64) * ops.E + 2.0 ** -20
+    far = ((x.double() - x.double().amax(1, keepdim=True)) / tau).abs()
+    eq = q * (sums + torch.where(q > 0, 8 * ops.E * far.clamp(max=200), 0.0) + 2.0 ** -17) + 1e-38
+    there = (ids >= 0) & (ids < V)
+    t = torch.where(there, top.double(), -math.inf) / tau
+    far_t = torch.where(p.sum(1, keepdim=True) > 0, (t.amax(1, keepdim=True) - t).clamp(max=200), 0.0).amax(1, keepdim=True)
+    ep = p * (2.0 ** -20 + 64 * ops.E + 8 * ops.E * far_t)
+    g = (dloss.double() * tau * any_)[:, None]
+    wx = g * (q - p)
+    tiny = 2.0 ** -25 if x.dtype == torch.float16 else 1e-38
+    ops.within(dx, wx, U * wx.abs() + g.abs() * (eq + ep + 2 * ops.E * (q + p)) + tiny, "dlogits")
+    ops.within(lse, want_lse, sums + 4 * ops.E * (x.double().amax(1) / tau).abs() + 4 * ops.E * want_lse.abs(), "lse")
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("V, k", [(33, 16), (33, 33), (64, 20), (65, 5), (1500, 32), (40000, 64)])
+@pytest.mark.parametrize("tau", [1e-6, 1e-3, 0.05, 1.0])
+def test_distill_gradient_at_low_temperatures_and_large_logits(m, kind, V, k, tau):
+    """Rows around 20, 1000 and 0, with the row's spread a few tau where the type has such differences, and tied maxima."""
+    T = 21
+    step = {"f32": 2.0 ** -19, "f16": 2.0 ** -6, "bf16": 2.0 ** -3}[kind]  # the last bit of numbers around 20
+    spread = max(step, tau)
+    x = 20.0 + (3 * ops.randn(300 + V, T, V) * spread / step).round() * step
+    x[::3] -= 20.0
+    x[1::3] += 980.0
+    x[5] = 20.0                     # all tied
+    x[6, 1:4] = x[6].max() + 8 * spread   # three tied maxima far above the rest
+    x = x.to(ops.KINDS[kind])
+    top, ids = (x.float() + 1.5 * spread * ops.randn(301, T, V)).topk(k, 1)
+    ids = ids.to(torch.int32)
+    if k > 2:
+        ids[1::4, k // 2:] = -1
+    dloss = ops.randn(302, T)
+    dloss[::5] = 0
+    got = ops.run_distill(m, x, ids, top.contiguous(), dloss / tau, tau)
+    check_soft(x, ids, top, dloss / tau, tau, *got)
+
+
+def test_distill_tied_maxima_share_their_probability(m):
+    for V in (33, 2000):
+        x = torch.full((3, V), -5.0, device="cuda")
+        x[:, 7] = x[:, 11] = 20.0
+        ids, top = torch.tensor([[3]] * 3, dtype=torch.int32, device="cuda"), torch.zeros(3, 1, device="cuda")
+        dloss = torch.full((3,), 1e6, device="cuda")
+        _, _, dx = ops.run_distill(m, x, ids, top, dloss, 1e-6)
+        want = torch.zeros(V, device="cuda")
+        want[7] = want[11] = 0.5
+        want[3] = -1.0
+        assert torch.allclose(dx, want.expand(3, V), rtol=1e-5, atol=0)
+
+
 # ---- errors that are found on the device --------------------------------------------------------------
 
 @pytest.fixture
