@@ -1891,6 +1891,12 @@ int check_logits(esm_ctx* c, int32_t type, int32_t T, int32_t V, int32_t k, int3
   return ESM_OK;
 }
 
+// Above 100 the loss, tau^2 times a sum that cancels to the order of tau^-2, has no digits left in fp32.
+int check_temperature(esm_ctx* c, float temperature) {
+  if (temperature >= 1e-6f && temperature <= 100.0f) return ESM_OK;
+  return fail(c, ESM_EINVAL, "distillation: the temperature must be in [1e-6, 100]");
+}
+
 int check_layernorm(esm_ctx* c, int32_t x_type, int32_t y_type, int32_t T, int32_t d) {
   if (!element_size(x_type) || !element_size(y_type)) return fail(c, ESM_EINVAL, "unknown element type");
   if (T < 0 || d <= 0 || d > kMaxSize / 2) return fail(c, ESM_EINVAL, "layernorm: bad number of rows or columns");
@@ -2121,8 +2127,8 @@ int esm_distill_loss(esm_ctx* c, int32_t type, const void* d_logits, int64_t ld,
   std::lock_guard<std::mutex> lk(c->mu);
   int rc = check_logits(c, type, T, V, k, 1);
   if (rc) return rc;
-  if (!(temperature >= 1e-6f && temperature <= 1e6f))
-    return fail(c, ESM_EINVAL, "distillation: the temperature must be in [1e-6, 1e6]");
+  rc = check_temperature(c, temperature);
+  if (rc) return rc;
   if (T == 0) return ESM_OK;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   DeviceScope dev(c->device);
@@ -2158,8 +2164,8 @@ int esm_distill_backward(esm_ctx* c, int32_t type, const void* d_logits, int64_t
   std::lock_guard<std::mutex> lk(c->mu);
   int rc = check_logits(c, type, T, V, k, 1);
   if (rc) return rc;
-  if (!(temperature >= 1e-6f && temperature <= 1e6f))
-    return fail(c, ESM_EINVAL, "distillation: the temperature must be in [1e-6, 1e6]");
+  rc = check_temperature(c, temperature);
+  if (rc) return rc;
   if (T == 0) return ESM_OK;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   DeviceScope dev(c->device);

@@ -347,7 +347,8 @@ int esm_score(esm_ctx* ctx, const int32_t* tokens, const int32_t* lengths, int32
  * (esm_token_logprobs' d_top_ids and d_top_logp of the teacher, or its logits at those ids): with
  * q = softmax(logits / temperature) over the vocabulary and p = softmax(top_logits / temperature) over
  * the row's alternatives,
- *   loss[t] = temperature^2 sum_i p_i (log p_i - log q[id_i]),  temperature in [1e-6, 1e6].
+ *   loss[t] = temperature^2 sum_i p_i (log p_i - log q[id_i]),  temperature in [1e-6, 100].
+ * The terms are taken in fp32, so the loss has an absolute error of up to temperature^2 2^-18 beside its rounding.
  * An alternative whose id is outside [0, V) is absent, and its d_top_logits entry is ignored; a row
  * without any (or with none above -inf) has loss 0. An id that is given twice counts with both its
  * probabilities. d_lse[t] = log sum_j exp(logits[t, j] / temperature), for the gradient. */

@@ -270,6 +270,35 @@ def test_distill_tied_maxima_share_their_probability(m):
         assert torch.allclose(dx, want.expand(3, V), rtol=1e-5, atol=0)
 
 
+@pytest.mark.parametrize("V", [33, 60, 500])
+@pytest.mark.parametrize("tau", [10.0, 100.0])
+def test_distill_loss_at_high_temperatures(m, V, tau):
+    """The loss tends to half the variance of the logits' differences: a sum of order tau^-2 of terms of order 1, whose
+    rounding is at most 2^-18: sums of V terms as in check_logprobs, two logarithms of at most log V, and their difference."""
+    k = min(V, 60)
+    x = 3 * ops.randn(310, 50, V)
+    x[:, k:] -= 1000.0 * tau          # only the alternatives count
+    ids = torch.arange(k, dtype=torch.int32, device="cuda").expand(50, k).contiguous()
+    top = (x[:, :k] + ops.randn(311, 50, k)).contiguous()
+    dloss = torch.ones(50, device="cuda")
+    loss, lse, dx = ops.run_distill(m, x, ids, top, dloss, tau)
+    want = ops.distill_64(x, ids, top, tau)[0]
+    ops.within(loss, want, tau * tau * 2.0 ** -18 + 8 * ops.E * want.abs(), "loss")
+    check_soft(x, ids, top, dloss, tau, loss, lse, dx)
+
+
+def test_distill_refuses_temperatures_that_fp32_does_not_support(esm, m):
+    x, ids, top, dloss = ops.distill_inputs(4, 33, 3, "f32", seed=99)
+    for tau in (1e-7, 9.9e-7, 100.1, 1e3, 1e6):
+        s, l = torch.full((4,), 7.0, device="cuda"), torch.full((4,), 7.0, device="cuda")
+        with pytest.raises(esm.EsmError, match="temperature must be in") as e:
+            m.distill_loss(x, ids, top, s, l, temperature=tau)
+        assert e.value.code == esm.ESM_EINVAL
+        with pytest.raises(esm.EsmError, match="temperature must be in"):
+            m.distill_backward(x, ids, top, l, dloss, torch.empty_like(x), temperature=tau)
+        assert (s == 7).all() and (l == 7).all()
+
+
 # ---- errors that are found on the device --------------------------------------------------------------
 
 @pytest.fixture
