@@ -27,7 +27,7 @@ constexpr int kSmallV = 64;
 // The distillation gradient takes q = exp(x / tau - lse) from the loss's lse while that is at most this large: the
 // rounding of lse and of x / tau is then at most 2^-17 of q (32 x 2^-24, four times). A row beyond it, for its logits or a low
 // temperature, takes its maximum and sum again, and subtracts the maximum first. 1021 x 32003 fp16: 29 us, and
-// 38 us with every row beyond it; 65536 x 33 fp32: 7.9 and 8.9.
+// 38 us with every row beyond it; 65536 x 33 fp32: 8.2 and 9.0.
 constexpr float kRoundedLse = 32.0f;
 
 // Keys that order like floats, -0 and +0 alike; 0 is below every number.
@@ -175,6 +175,7 @@ struct QuadTeacher {
   }
   __device__ __forceinline__ void normalise(int V, float inv_tau) {
     float top = -INFINITY, s = 0.0f;
+    bool there = false;  // a NaN is not dropped by this as by the maximum: it has to show in the loss
 #pragma unroll
     for (int c = 0; c < K; ++c) {
       if (id[c] < 0 || id[c] >= V) {
@@ -182,9 +183,10 @@ struct QuadTeacher {
         v[c] = -INFINITY;
       }
       top = fmaxf(top, v[c]);
+      there |= v[c] != -INFINITY;
     }
     top = quad_max(top);
-    any = top > -INFINITY;
+    any = quad_max(there) > 0.0f;
 #pragma unroll
     for (int c = 0; c < K; ++c) {
       v[c] = (v[c] - top) * inv_tau;
@@ -509,6 +511,7 @@ __device__ __forceinline__ bool teacher(const LogitsOp& p, int64_t t, int lane, 
     v[c] = id[c] >= 0 ? p.alt_logits[t * p.k + i] : -INFINITY;
     m = fmaxf(m, v[c]);
   }
+  const bool any = __any_sync(0xffffffffu, v[0] != -INFINITY || v[1] != -INFINITY);  // NaN too: it has to show
   m = warp_max(m);
   float s = 0.0f;
 #pragma unroll
@@ -519,7 +522,7 @@ __device__ __forceinline__ bool teacher(const LogitsOp& p, int64_t t, int lane, 
     logp[c] = (v[c] - m) * inv_tau - log_s;
     pr[c] = id[c] >= 0 ? fast_exp2(logp[c] * kLog2e) : 0.0f;
   }
-  return m > -INFINITY;
+  return any;
 }
 
 // 1021 x 32003 fp16: loss 20 us, gradient 25 (22 and 27 on cold caches: 3.0 and 4.8 TB/s). The loss is bound by its

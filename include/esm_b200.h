@@ -350,7 +350,7 @@ int esm_score(esm_ctx* ctx, const int32_t* tokens, const int32_t* lengths, int32
  *   loss[t] = temperature^2 sum_i p_i (log p_i - log q[id_i]),  temperature in [1e-6, 100].
  * The terms are taken in fp32, so the loss has an absolute error of up to temperature^2 2^-18 beside its rounding.
  * An alternative whose id is outside [0, V) is absent, and its d_top_logits entry is ignored; a row
- * without any (or with none above -inf) has loss 0. An id that is given twice counts with both its
+ * without any (or with nothing but -inf) has loss 0; a NaN shows in the loss and gradient. An id that is given twice counts with both its
  * probabilities. d_lse[t] = log sum_j exp(logits[t, j] / temperature), for the gradient. */
 int esm_distill_loss(esm_ctx* ctx, int32_t type, const void* d_logits, int64_t ld, int32_t T, int32_t V,
                      const int32_t* d_top_ids, const float* d_top_logits, int32_t k, float temperature, float* d_loss,

@@ -299,6 +299,25 @@ def test_distill_refuses_temperatures_that_fp32_does_not_support(esm, m):
         assert (s == 7).all() and (l == 7).all()
 
 
+@pytest.mark.parametrize("V", [33, 50, 300, 5000])
+@pytest.mark.parametrize("k", [1, 3, 20, 33])
+def test_distill_a_teacher_of_nan_alone_shows(m, V, k):
+    """Rows whose present alternatives are all NaN, or NaN and -inf, are not rows without alternatives."""
+    x = ops.logits_of(6, V, "f32", seed=320)
+    ids = torch.arange(k, dtype=torch.int32, device="cuda").expand(6, k).contiguous()
+    top = torch.full((6, k), math.nan, device="cuda")
+    top[1, 1:] = -math.inf
+    ids[2, : k - 1] = -1
+    top[3] = 0.5
+    top[4] = -math.inf
+    ids[5] = V
+    loss, lse, dx = ops.run_distill(m, x, ids, top, torch.ones(6, device="cuda"), 2.0)
+    assert torch.isnan(loss[:3]).all() and torch.isfinite(loss[3]) and (loss[4:] == 0).all()
+    for row in range(3):
+        assert torch.isnan(dx[row, ids[row][ids[row] >= 0].long()]).any()
+    assert torch.isfinite(dx[3]).all() and (dx[4:] == 0).all() and torch.isfinite(lse).all()
+
+
 # ---- errors that are found on the device --------------------------------------------------------------
 
 @pytest.fixture
