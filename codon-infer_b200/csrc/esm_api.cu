@@ -1829,6 +1829,16 @@ struct Buffer {
   }
 };
 
+// Whether two buffers share memory. Blocks of columns of one matrix, whose address ranges interlock, do not: with the
+// same distance P between their rows, a's rows are [0, wa) and b's [d, d + wb) modulo P.
+bool overlap(const Buffer& a, const Buffer& b) {
+  if (!(a.begin() < b.end() && b.begin() < a.end())) return false;
+  const uintptr_t pitch = a.ld * a.size, wa = a.cols * a.size, wb = b.cols * b.size;
+  if (a.rows == 1 || b.rows == 1 || pitch != b.ld * b.size) return true;
+  const uintptr_t d = b.begin() >= a.begin() ? (b.begin() - a.begin()) % pitch : (pitch - (a.begin() - b.begin()) % pitch) % pitch;
+  return d < wa || d + wb > pitch;
+}
+
 // Every buffer given, aligned, on the context's device, rows not overlapping, and none that is
 // written shares memory with another one.
 int check_buffers(esm_ctx* c, const Buffer* b, int n, cudaStream_t s) {
@@ -1863,7 +1873,7 @@ int check_buffers(esm_ctx* c, const Buffer* b, int n, cudaStream_t s) {
   }
   for (int i = 0; i < n; ++i)
     for (int j = i + 1; j < n; ++j)
-      if (b[i].p && b[j].p && (b[i].written || b[j].written) && b[i].begin() < b[j].end() && b[j].begin() < b[i].end())
+      if (b[i].p && b[j].p && (b[i].written || b[j].written) && overlap(b[i], b[j]))
         return fail(c, ESM_EINVAL, std::string(b[i].name) + " and " + b[j].name + " overlap");
   return ESM_OK;
 }

@@ -257,7 +257,8 @@ int esm_matmul_tiled_noalloc(int32_t dtype, const float* d_x, const void* d_w, c
  * are row strides in elements. A call is enqueued on `stream` (a cudaStream_t of that GPU; NULL =
  * the legacy default stream), allocates nothing and does not wait, so it may be captured into a CUDA
  * graph; it does not change the calling thread's current device. A null, misaligned, foreign-device
- * or host pointer, or a buffer that is written and overlaps another one, is ESM_EINVAL; a workspace
+ * or host pointer, or a buffer that is written and overlaps another one, is ESM_EINVAL (column blocks of one
+ * matrix may be separate buffers; buffers with other row strides overlap when their address ranges do); a workspace
  * that is too small is ESM_ECAPACITY. A workspace holds nothing between calls; calls that may run
  * at the same time (two streams, two captured graphs) need one each. Results do not depend on how
  * often or beside what a call runs: sums are taken in a fixed order. What an operator finds wrong on the device is

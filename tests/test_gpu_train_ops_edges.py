@@ -318,6 +318,58 @@ def test_distill_a_teacher_of_nan_alone_shows(m, V, k):
     assert torch.isfinite(dx[3]).all() and (dx[4:] == 0).all() and torch.isfinite(lse).all()
 
 
+# ---- layouts ------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("T", [1, 2, 77])
+def test_attention_on_column_blocks_of_one_matrix(m, T):
+    """qkv, out, dout and dqkv side by side in one matrix: their address ranges interlock, their elements do not."""
+    H, dh = 2, 24
+    d = H * dh
+    cu, qkv, dout = ops.attention_inputs([T], H, dh, "f16", seed=400)
+    out, lse = ops.run_forward(m, cu, qkv, H, T)
+    dqkv = ops.run_backward(m, cu, qkv, H, T, out, lse, dout)
+    store = torch.full((T, 8 * d + 8), 7.0, dtype=torch.float16, device="cuda")
+    out2, qkv2, dqkv2, dout2 = store[:, :d], store[:, d:4 * d], store[:, 4 * d:7 * d], store[:, 7 * d:8 * d]
+    qkv2.copy_(qkv), dout2.copy_(dout)
+    lse2 = torch.empty_like(lse)
+    ws = torch.empty(m.attention_backward_workspace(1, T, H), dtype=torch.uint8, device="cuda")
+    m.attention(qkv2, cu, T, H, out2, lse2)
+    m.attention_backward(qkv2, cu, T, H, out2, lse2, dout2, dqkv2, ws)
+    assert torch.equal(out2, out) and torch.equal(lse2, lse) and torch.equal(dqkv2, dqkv)
+    assert torch.equal(qkv2, qkv) and torch.equal(dout2, dout) and (store[:, 8 * d:] == 7.0).all()
+
+
+def test_distill_gradient_beside_the_logits(m):
+    x, ids, top, dloss = ops.distill_inputs(40, 33, 5, "f32", seed=401)
+    want = ops.run_distill(m, x, ids, top, dloss, 1.0)
+    store = torch.full((40, 70), 7.0, device="cuda")
+    grad, logits = store[:, 1:34], store[:, 34:67]
+    logits.copy_(x)
+    loss, lse = torch.empty(40, device="cuda"), torch.empty(40, device="cuda")
+    m.distill_loss(logits, ids, top, loss, lse)
+    m.distill_backward(logits, ids, top, lse, dloss, grad)
+    assert torch.equal(grad, want[2]) and torch.equal(logits, x) and (store[:, 0] == 7).all() and (store[:, 67:] == 7).all()
+
+
+def test_column_blocks_that_share_elements_are_refused(m, esm):
+    T, V = 9, 33
+    x, ids, top, dloss = ops.distill_inputs(T, V, 5, "f32", seed=402)
+    lse = torch.zeros(T, device="cuda")
+    store = torch.zeros(T + 2, 70, device="cuda")
+
+    def refused(logits, grad):
+        for a, b in ((logits, grad), (grad, logits)):
+            with pytest.raises(esm.EsmError, match="overlap") as e:
+                m.distill_backward(a, ids, top, lse, dloss, b)
+            assert e.value.code == esm.ESM_EINVAL
+
+    rows = store[:T]
+    refused(rows[:, :33], rows[:, 32:65])                 # one column in common
+    refused(rows[:, :33], store[1:T + 1, 20:53])          # the same, a row further
+    refused(rows[:, :33], store.view(-1)[70 + 52:].as_strided((T, 33), (70, 1)))   # its row's end meets the next row's start
+    refused(rows[:, :33], store.view(-1)[37:].as_strided((T, 33), (69, 1)))          # other strides: not told apart
+
+
 # ---- errors that are found on the device --------------------------------------------------------------
 
 @pytest.fixture
