@@ -1892,6 +1892,9 @@ int check_attention(esm_ctx* c, int32_t type, int32_t B, int32_t T, int32_t max_
   return ESM_OK;
 }
 
+// The stride of a single row says nothing, and need not be one that a tensor map takes.
+int64_t row_stride(int32_t rows, int64_t ld, int64_t cols) { return rows > 1 ? ld : cols; }
+
 int check_logits(esm_ctx* c, int32_t type, int32_t T, int32_t V, int32_t k, int32_t k_min) {
   if (!element_size(type)) return fail(c, ESM_EINVAL, "unknown element type");
   if (T < 0 || V <= 0 || V > kMaxSize) return fail(c, ESM_EINVAL, "bad number of rows or vocabulary size");
@@ -1936,7 +1939,7 @@ int esm_attention(esm_ctx* c, int32_t type, const void* d_qkv, int64_t ld_qkv, c
   esm::AttnOp p{};
   p.dtype = type;
   p.qkv = d_qkv;
-  p.ld_qkv = ld_qkv;
+  p.ld_qkv = row_stride(T, ld_qkv, 3 * d);
   p.cu = d_cu_seqlens;
   p.B = B;
   p.T = T;
@@ -1945,7 +1948,7 @@ int esm_attention(esm_ctx* c, int32_t type, const void* d_qkv, int64_t ld_qkv, c
   p.dh = head_dim;
   p.scale = scale;
   p.out = d_out;
-  p.ld_out = ld_out;
+  p.ld_out = row_stride(T, ld_out, d);
   p.lse = d_lse;
   p.err = c->d_err + 1;
   ESM_CUDA(esm::launch_attention_op(p, s));
@@ -1986,7 +1989,7 @@ int esm_attention_backward(esm_ctx* c, int32_t type, const void* d_qkv, int64_t 
   esm::AttnOp p{};
   p.dtype = type;
   p.qkv = d_qkv;
-  p.ld_qkv = ld_qkv;
+  p.ld_qkv = row_stride(T, ld_qkv, 3 * d);
   p.cu = d_cu_seqlens;
   p.B = B;
   p.T = T;
@@ -1995,12 +1998,12 @@ int esm_attention_backward(esm_ctx* c, int32_t type, const void* d_qkv, int64_t 
   p.dh = head_dim;
   p.scale = scale;
   p.out = const_cast<void*>(d_out);
-  p.ld_out = ld_out;
+  p.ld_out = row_stride(T, ld_out, d);
   p.lse = const_cast<float*>(d_lse);
   p.dout = d_dout;
-  p.ld_dout = ld_dout;
+  p.ld_dout = row_stride(T, ld_dout, d);
   p.dqkv = d_dqkv;
-  p.ld_dqkv = ld_dqkv;
+  p.ld_dqkv = row_stride(T, ld_dqkv, 3 * d);
   p.workspace = static_cast<float*>(d_workspace);
   p.num_sms = c->num_sms;
   p.err = c->d_err + 1;

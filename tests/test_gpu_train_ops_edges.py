@@ -339,6 +339,28 @@ def test_attention_on_column_blocks_of_one_matrix(m, T):
     assert torch.equal(qkv2, qkv) and torch.equal(dout2, dout) and (store[:, 8 * d:] == 7.0).all()
 
 
+def test_attention_of_one_row_takes_any_stride(m, esm):
+    """No second row starts anywhere: the stride need not be a multiple of 16 bytes."""
+    H, dh = 2, 8
+    d = H * dh
+    cu, qkv, dout = ops.attention_inputs([1], H, dh, "f16", seed=403)
+    out, lse = ops.run_forward(m, cu, qkv, H, 1)
+    dqkv = ops.run_backward(m, cu, qkv, H, 1, out, lse, dout)
+    L, scale = esm.lib(), dh ** -0.5
+    out2, lse2, dqkv2 = torch.zeros_like(out), torch.zeros_like(lse), torch.zeros_like(dqkv)
+    size = m.attention_backward_workspace(1, 1, H)
+    ws = torch.empty(size, dtype=torch.uint8, device="cuda")
+    for odd in (1, 3, 2 ** 33 + 1):
+        rc = L.esm_attention(m._ctx, esm.TYPE_F16, qkv.data_ptr(), 3 * d + odd, cu.data_ptr(), 1, 1, 1, H, dh, scale,
+                             out2.data_ptr(), d + odd, lse2.data_ptr(), None)
+        assert rc == esm.ESM_OK, L.esm_last_error(m._ctx).decode()
+        rc = L.esm_attention_backward(m._ctx, esm.TYPE_F16, qkv.data_ptr(), 3 * d + odd, cu.data_ptr(), 1, 1, 1, H, dh, scale,
+                                      out2.data_ptr(), d + odd, lse2.data_ptr(), dout.data_ptr(), d + odd, dqkv2.data_ptr(),
+                                      3 * d + odd, ws.data_ptr(), size, None)
+        assert rc == esm.ESM_OK, L.esm_last_error(m._ctx).decode()
+        assert torch.equal(out2, out) and torch.equal(lse2, lse) and torch.equal(dqkv2, dqkv)
+
+
 def test_distill_gradient_beside_the_logits(m):
     x, ids, top, dloss = ops.distill_inputs(40, 33, 5, "f32", seed=401)
     want = ops.run_distill(m, x, ids, top, dloss, 1.0)
