@@ -26,6 +26,7 @@
 // O is rescaled in tensor memory only when the running max has gone stale (EXP 3, the default: a
 // step's row sum against it exceeds p.rescale_sum; EXP 0..2: a step's row max exceeds it by more
 // than 2^8), after PV(j - 1) has completed. All waits are bounded.
+#include <algorithm>
 #include <atomic>
 #include <type_traits>
 
@@ -652,7 +653,7 @@ cudaError_t launch_op(const CUtensorMap& tm_q, const CUtensorMap& tm_kv, const A
   static std::atomic<unsigned long long> configured{0};
   cudaError_t e = allow_smem(kernel, kSmem, configured);
   if (e != cudaSuccess) return e;
-  kernel<<<dim3((p.max_len + 2 * kQ - 1) / (2 * kQ), p.H, B), kThreads3, kSmem, s>>>(tm_q, tm_kv, tm_q, tm_kv, p);
+  kernel<<<dim3(std::max(1, (p.max_len + 2 * kQ - 1) / (2 * kQ)), p.H, B), kThreads3, kSmem, s>>>(tm_q, tm_kv, tm_q, tm_kv, p);
   return cudaGetLastError();
 }
 

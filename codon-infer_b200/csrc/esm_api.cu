@@ -1925,7 +1925,7 @@ int esm_attention(esm_ctx* c, int32_t type, const void* d_qkv, int64_t ld_qkv, c
   std::lock_guard<std::mutex> lk(c->mu);
   int rc = check_attention(c, type, B, T, max_len, n_heads, head_dim, scale);
   if (rc) return rc;
-  if (B == 0 || T == 0 || max_len == 0) return ESM_OK;
+  if (B == 0 || T == 0) return ESM_OK;  // max_len = 0: the launch looks whether the sequences are empty
   const int64_t d = static_cast<int64_t>(n_heads) * head_dim;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   DeviceScope dev(c->device);
@@ -1969,7 +1969,7 @@ int esm_attention_backward(esm_ctx* c, int32_t type, const void* d_qkv, int64_t 
   std::lock_guard<std::mutex> lk(c->mu);
   int rc = check_attention(c, type, B, T, max_len, n_heads, head_dim, scale);
   if (rc) return rc;
-  if (B == 0 || T == 0 || max_len == 0) return ESM_OK;
+  if (B == 0 || T == 0) return ESM_OK;  // max_len = 0: the launch looks whether the sequences are empty
   const size_t need = esm::attention_backward_bytes(B, T, n_heads);
   if (workspace_bytes < need)
     return fail(c, ESM_ECAPACITY, "attention backward needs a workspace of " + std::to_string(need) + " bytes");

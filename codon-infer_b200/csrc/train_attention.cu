@@ -745,7 +745,8 @@ cudaError_t backward(const AttnOp& a, const BwdParams& p, cudaStream_t s) {
   static std::atomic<unsigned long long> configured{0};
   cudaError_t e = allow_smem(attention_backward_kernel<DH, E>, Bwd<DH>::kSmem, configured);
   if (e != cudaSuccess) return e;
-  attention_delta_kernel<E><<<dim3((a.max_len + kDeltaRows - 1) / kDeltaRows, a.H, a.B), 256, 0, s>>>(p);
+  attention_delta_kernel<E><<<dim3(std::max(1, (a.max_len + kDeltaRows - 1) / kDeltaRows), a.H, a.B), 256, 0, s>>>(p);
+  if (a.max_len == 0) return cudaGetLastError();  // only the offsets were looked at
   const int64_t items = static_cast<int64_t>(2) * (a.T / kOwn + a.B) * a.H;  // at most
   attention_backward_kernel<DH, E>
       <<<static_cast<unsigned>(std::min<int64_t>(items, a.num_sms)), kThreads, Bwd<DH>::kSmem, s>>>(tm_qkv, tm_dout, tm_qkv_own,

@@ -451,3 +451,20 @@ def test_errors_of_several_calls_are_all_named(esm, encoder):
     message = esm.lib().esm_last_error(encoder._ctx).decode()
     assert "wait gave up" in message and "token id" in message
     encoder.check_device()
+
+
+def test_a_bound_of_no_rows_is_checked_like_any_other(esm, m):
+    """max_len = 0 with sequences that are not empty: they are longer than max_len, and esm_check_device says so."""
+    cu, qkv, dout = ops.attention_inputs([3, 0, 61], 2, 16, "f16", seed=420)
+    out, lse = ops.run_forward(m, cu, qkv, 2, 64)
+    m.check_device()
+    out0, lse0 = ops.run_forward(m, cu, qkv, 2, 0)
+    assert (out0 == 7).all() and (lse0 == 7).all()
+    with pytest.raises(esm.EsmError, match="cu_seqlens"):
+        m.check_device()
+    assert (ops.run_backward(m, cu, qkv, 2, 0, out, lse, dout) == 7).all()
+    with pytest.raises(esm.EsmError, match="cu_seqlens"):
+        m.check_device()
+    cu.fill_(64)
+    ops.run_backward(m, cu, qkv, 2, 0, *ops.run_forward(m, cu, qkv, 2, 0), dout)
+    m.check_device()
