@@ -192,6 +192,19 @@ def test_attention_backward_of_large_sums(m, kind, terms):
     ops.check_backward(cu, qkv, 1, out, lse, dout, dqkv)
 
 
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("lens", [[1, 5, 31, 32, 33], [257, 64], [700]], ids=str)
+def test_attention_exponentials_are_exact_to_32_bits(m, monkeypatch, kind, lens):
+    """The bounds of the helpers with what the operator's exponentials have: 2^-21, the exp2 instruction's 2^-22 or
+    the polynomial's 2.2e-7 with their rounding, and sums of 32 of a row's columns at a time, then over the steps."""
+    monkeypatch.setattr(ops, "X", 2.0 ** -21 + (32 + 3 * max(lens) / 32) * ops.E)
+    for H, dh in ((3, 64), (2, 24)):
+        cu, qkv, dout = ops.attention_inputs(lens, H, dh, kind, seed=250 + dh)
+        out, lse = ops.run_forward(m, cu, qkv, H, max(lens))
+        ops.check_forward(cu, qkv, H, out, lse)
+        ops.check_backward(cu, qkv, H, out, lse, dout, ops.run_backward(m, cu, qkv, H, max(lens), out, lse, dout))
+
+
 @pytest.mark.parametrize("dim, heads", [(640, 10), (320, 20)])
 def test_encoder_forward_of_a_short_sequence_with_nan(esm, dim, heads):
     """The encoder's own attention: heads of 64 and of 16 columns, 1 to 33 tokens, one of them NaN."""
