@@ -46,6 +46,25 @@ def test_attention_bad_rows_of_short_sequences_are_written(m, kind, bad):
 
 
 @pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_attention_backward_of_bad_short_sequences_stays_alone(m, kind, bad):
+    """Gradients of a spoiled sequence are not finite, and those of its neighbours what they were."""
+    for H, dh in ((2, 64), (3, 24)):
+        lens = [70, 1, 20, 31, 32, 33, 64, 65, 40]
+        cu, qkv, dout = ops.attention_inputs(lens, H, dh, kind, seed=260 + dh)
+        c, d = cu.tolist(), H * dh
+        out, lse = ops.run_forward(m, cu, qkv, H, 70)
+        dqkv = ops.run_backward(m, cu, qkv, H, 70, out, lse, dout)
+        qkv2 = qkv.clone()
+        qkv2[c[1]:c[8], d:] = bad                     # keys and values
+        out2, lse2 = ops.run_forward(m, cu, qkv2, H, 70)
+        dqkv2 = ops.run_backward(m, cu, qkv2, H, 70, out2, lse2, dout)
+        m.check_device()
+        assert torch.equal(dqkv2[:c[1]], dqkv[:c[1]]) and torch.equal(dqkv2[c[8]:], dqkv[c[8]:])
+        assert not torch.isfinite(dqkv2[c[1]:c[8]]).any()
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
 @pytest.mark.parametrize("bad", [math.nan, math.inf])
 def test_attention_a_bad_key_shows_in_every_row(m, kind, bad):
     """One key of one head is not finite, at every place of the first and of a later key tile: every query of that
