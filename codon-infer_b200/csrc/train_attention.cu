@@ -17,9 +17,10 @@
 // One persistent block per SM takes items from a list (see the producer). Tensor memory (512 columns): three score
 // buffers of 128 columns (S in the first 64, dP in the other 64), acc1 and acc2. Step n uses buffer n % 3, so
 // the tensor cores compute the next steps' scores and the last one's products while the elementwise warps
-// work on a step. P and dS go back over S and dP as 16-bit pairs (each warp over the first half of the 16
+// work on a step. P and dS go back over S and dP as 16-bit pairs (each warp over the first half of the 32
 // columns it read) and are read from there as the A operand.
-//   warps 0..15  elementwise: a warp has 32 owned rows and 16 of the 64 columns of every step
+//   warps 0..15  elementwise, in two teams of eight that take every other step: a warp has 32 owned rows and 32 of
+//                the step's 64 columns
 //   warps 16..19 store an item's gradients while the others go on with the next item
 //   warp 20      producer: finds items, loads their operands (two slots) and the stream (TMA ring)
 //   warp 23      splits lse and D of the streamed queries of key items (below), and clears the rows behind a
@@ -43,14 +44,16 @@
 // fp16: P and dS are scaled by powers of two before they are rounded, P by 2^14 in key items and dS
 // by 2^e with 2^e * 2 dh max|dO| max|V| <= 2^14, which bounds it; the outputs are scaled back in fp32.
 //
-// Measured: 16 x 1024 tokens of 20 x 64 heads, fp16, 358 us in all, 25 of them attention_delta_kernel (126 MB);
-// 2 x 4096 of 40 x 64, bf16, 1.34 ms. What bounds it: at 16 x 1024 a step of 64 x 128 takes 1180 cycles. With the
-// elementwise work left out it takes 285 us of 361, with the tensor cores' 306, with both 261, and without the
-// split of lse and D 189: the stages are about as long as one another, and none alone is the bound. Tried
-// and slower or no faster: two blocks per SM that are not persistent (518), one issuer for all MMAs (447),
-// 128-row streamed tiles (357, but 8 to 16 % more on short sequences), 8 elementwise warps (392), barriers of their
-// own for S and dP (375), a second pair of accumulators, exponentials partly on the FP32 pipe, lse and D loaded
-// four steps ahead, and for DH 32 16-byte copies by the producer warp instead of TMA (140 -> 167 at 32 x 64..512).
+// Measured, in bursts at 1965 MHz: 16 x 1024 tokens of 20 x 64 heads, fp16, 358 us in all, 25 of them
+// attention_delta_kernel (126 MB); 2 x 4096 of 40 x 64, bf16, 1.21 ms. Call after call the power cap sets the clock:
+// 418 us at 1560 MHz and 1.39 ms at 1665. What bounds it: a step of 64 x 128 takes 1180 cycles. With the elementwise
+// arithmetic left out the 358 us become 315, with the MMAs left out 295, with both 259, with the split of lse and D
+// left out 355, and with all three 211: the stages are about as long as one another, and none alone is the
+// bound. The kernel is at its limit of 80 registers; DH 64 spills 44 (bf16) and 64 bytes (fp16), DH 32 none. Tried
+// and slower or no faster: two blocks per SM that are not persistent (518), one issuer for all MMAs (447), 128-row
+// streamed tiles (357, but 8 to 16 % more on short sequences), 8 elementwise warps (392), barriers of their own for
+// S and dP (375), a second pair of accumulators, exponentials partly on the FP32 pipe, lse and D loaded four steps
+// ahead, and for DH 32 16-byte copies by the producer warp instead of TMA (140 -> 167 at 32 x 64..512).
 #include "common.cuh"
 #include "gemm_tc.cuh"
 #include "train_common.cuh"
@@ -647,9 +650,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
   } else {
-    // ---------------- elementwise: one owned row per thread, 16 of the 64 columns ----------------
-    // All 16 warps share every step: a step's latency from its scores to its products bounds the loop (three
-    // are in flight), not the special-function unit, which takes 512 cycles a step for the exponentials.
+    // ---------------- elementwise: one owned row per thread, 32 of the 64 columns ----------------
+    // Eight warps a step, and two teams that take steps in turn: three steps are in flight, and one team's wait for
+    // scores, and its reads and writes of tensor memory, pass behind the other's arithmetic. The special-function
+    // unit takes 512 cycles a step for the exponentials, less than half of it.
     const int quarter = warp & 3, team = warp / kTeamWarps, cols = kWarpCols * (warp % kTeamWarps >> 2);
     const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + cols;
     const float c = p.scale * kLog2e;

@@ -199,7 +199,7 @@ struct QuadTeacher {
   __device__ __forceinline__ float prob(int c) const { return id[c] >= 0 ? fast_exp2(v[c] * kLog2e) : 0.0f; }
 };
 
-// 65536 x 33 fp32, k up to 16: loss 7.6 us, gradient 10.4 (9.6 and 12.4 on cold caches); issue 52 and 58 %.
+// 65536 x 33 fp32, k up to 16: loss 6.4 us, gradient 8.2 (8.7 and 10.9 on cold caches); issue 52 and 64 %.
 template <typename E, int N, int K>
 __global__ void __launch_bounds__(128) distill_loss_quad_kernel(const LogitsOp p) {
   const QuadRow r(p.T);
@@ -525,7 +525,7 @@ __device__ __forceinline__ bool teacher(const LogitsOp& p, int64_t t, int lane, 
   return any;
 }
 
-// 1021 x 32003 fp16: loss 20 us, gradient 25 (22 and 27 on cold caches: 3.0 and 4.8 TB/s). The loss is bound by its
+// 1021 x 32003 fp16: loss 16 us, gradient 29 (21 and 26 on cold caches: 3.1 and 5.0 TB/s). The loss is bound by its
 // exponentials (special-function unit 53 %) and a row's latency, the gradient by the latter.
 template <int NT, typename E>
 __global__ void __launch_bounds__(NT) distill_loss_row_kernel(const LogitsOp p) {
@@ -618,10 +618,17 @@ __global__ void __launch_bounds__(NT) distill_backward_row_kernel(const LogitsOp
 
 unsigned quads(const LogitsOp& p) { return (static_cast<unsigned>(p.T) + 31) / 32; }
 
-// Threads of a row's block: one warp for short rows; for long ones 512, or 256 where there are more rows than
-// 512-thread blocks fit the GPU at once (4 x 148). Loss of 1021 x 32003 fp16: 20 us with 256, 27 us with 512. What
-// bounds these is the latency of a row's passes: copying rows to shared memory in bulk, or starting from the
-// maximum of a row's first vectors so that the running maximum seldom rises, was no faster.
+// Threads of a row's block, by its length: few rows want many threads, many rows want few. Log probabilities
+// without a top k / distillation loss, fp16, us:
+//   1024 tokens, 16384 rows: 32 threads 16.8 / 15.2, 128 29.8 / 28.6; 400 rows: 3.9 / 4.2 and 3.3 / 3.8
+//   2048 tokens, 8192 rows: 32 threads 14.4 / 12.4, 128 19.7 / 18.4; 400 rows: 5.3 / 5.7 and 3.7 / 4.5
+//   6000 tokens, 2796 rows: 128 threads 13.9 / 11.9, 256 16.8 / 14.8; 400 rows: 128 5.4 / 5.3, 512 6.2 / 6.0
+//   32768 tokens, 512 rows: 256 threads 12.5 / 11.2, 512 13.5 / 11.8 (gradient 11.5 and 10.9); 1021 x 32003 loss: 256
+//   20 us, 512 27. 592 is how many 512-thread blocks fit the GPU at once.
+// So 128 threads from 1025 tokens and 256 or 512 from 4097 are up to a third slower with many rows and about as much
+// faster, or even, with few. What bounds the long rows is the latency of a row's passes: copying rows to shared
+// memory in bulk, or starting from the maximum of a row's first vectors so that the running maximum seldom rises,
+// was no faster.
 int row_block(const LogitsOp& p) {
   if (p.V <= 1024) return 32;
   if (p.V <= 4096) return 128;
@@ -633,7 +640,10 @@ cudaError_t logprobs(const LogitsOp& p, cudaStream_t s) {
   const int nt = row_block(p);
   if (p.V <= 40) logprobs_quad_kernel<E, 10><<<quads(p), 128, 0, s>>>(p);
   else if (p.V <= kSmallV) logprobs_quad_kernel<E, 16><<<quads(p), 128, 0, s>>>(p);
-  else if (nt == 32 && p.k <= 16) logprobs_row_kernel<32, E><<<p.T, 32, 0, s>>>(p);  // a warp's 32 maxima bound the top k
+  // One warp's 32 maxima bound the top 16 well: 32768 x 512 fp16, k = 5: 44 us. With more alternatives, or with 128
+  // threads, rows of up to about 900 16-bit or 450 fp32 elements leave a warp without enough maxima, the bound is 0, and
+  // every element is ranked against all others: 1395 us with k = 32, and 1386 with k = 5 and 128 threads.
+  else if (nt == 32 && p.k <= 16) logprobs_row_kernel<32, E><<<p.T, 32, 0, s>>>(p);
   else if (nt <= 128) logprobs_row_kernel<128, E><<<p.T, 128, 0, s>>>(p);
   else if (nt == 256) logprobs_row_kernel<256, E><<<p.T, 256, 0, s>>>(p);
   else logprobs_row_kernel<512, E><<<p.T, 512, 0, s>>>(p);

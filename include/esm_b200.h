@@ -249,11 +249,12 @@ int esm_matmul_tiled_noalloc(int32_t dtype, const float* d_x, const void* d_w, c
 
 /* ---- training and scoring operators on device memory (no counterpart in the reference) --------- */
 
-/* What a distillation or fine-tuning step of the encoder needs around its GEMMs: attention over
+/* Operators that a distillation or fine-tuning step of the encoder has beside its GEMMs: attention over
  * packed sequences with its backward pass, LayerNorm with its backward pass, per-token log
- * probabilities, and the loss of a student against a teacher's top alternatives with its gradient.
+ * probabilities, and the loss of a student against a teacher's top alternatives with its gradient. (The
+ * gradients of GELU and of rotary positions, and a forward that keeps what a backward pass needs, are not here.)
  *
- * All of them: buffers are DEVICE memory of the context's GPU, rows are row-major, `ld` arguments
+ * All of them but esm_score, a host call like esm_forward: buffers are DEVICE memory of the context's GPU, rows are row-major, `ld` arguments
  * are row strides in elements. A call is enqueued on `stream` (a cudaStream_t of that GPU; NULL =
  * the legacy default stream), allocates nothing and does not wait, so it may be captured into a CUDA
  * graph; it does not change the calling thread's current device. A null, misaligned, foreign-device
@@ -279,10 +280,11 @@ enum { ESM_F32 = 0, ESM_F16 = 1, ESM_BF16 = 2 };
  * rows of the buffers: rows behind the last sequence are left as they are. head_dim is a multiple of 8
  * up to 64, scale in [1e-6, 1e6]; B and n_heads are at most 65535, T at most 2^30. d_lse [H, T] or NULL (the
  * backward pass needs it). Scores, sums and outputs are accumulated in fp32, probabilities are rounded to
- * `type` for the product with V. A row with a score that is NaN or +inf has NaN in out and lse; scores of -inf have
- * probability 0, and a row with no other has NaN in out and lse -inf; finite q k are at most 1e30 in
- * magnitude. Offsets that do not fit (descending, beyond T or longer than max_len) are noticed on the device: that sequence, and in the backward pass perhaps others, is skipped and
- * esm_check_device returns ESM_EINVAL. */
+ * `type` for the product with V. A row with a score that is NaN or +inf has NaN in out and lse; scores of -inf
+ * have probability 0 (their infinite keys still make dQ NaN in the backward pass), and a row with no other has NaN
+ * in out and lse -inf; finite q k are at most 1e30 in magnitude. Offsets that do not fit (descending, beyond T or
+ * longer than max_len) are noticed on the device: that sequence, and in the backward pass perhaps others, is
+ * skipped and esm_check_device returns ESM_EINVAL. */
 int esm_attention(esm_ctx* ctx, int32_t type, const void* d_qkv, int64_t ld_qkv, const int32_t* d_cu_seqlens,
                   int32_t B, int32_t T, int32_t max_len, int32_t n_heads, int32_t head_dim, float scale, void* d_out,
                   int64_t ld_out, float* d_lse, void* stream);
