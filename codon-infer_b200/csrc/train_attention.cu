@@ -34,7 +34,7 @@
 // shared-memory bandwidth than all operand reads of the tensor cores (a 16-byte broadcast read is four
 // wavefronts), so they are subtracted by the tensor cores: one more K step of 16 with constants in every row of
 // A, (2^15, 2^3, 2^-9) for fp16 and ones for bf16, and -lse / scale, or -D, split into three parts of the
-// operand type in B. For fp16 that covers magnitudes up to 2^30, to 2^-34 or 2^-24 relative.
+// operand type in B. For fp16 that covers magnitudes up to 2^30, to 2^-22 relative or better, or 2^-34.
 //
 // Heads narrower than 32 or 64 columns arrive zero-padded by the 3-D tensor maps. Rows past the
 // sequence's end in the last streamed tile are cleared in shared memory (they belong to other
@@ -197,11 +197,14 @@ __device__ __forceinline__ int ds_exponent(const BwdParams& p, int start, int le
 // x as three values of E, times 2^15, 2^3 and 2^-9 for fp16 (whose range the factors extend) and 1
 // for bf16, packed into the first 16 bytes of a K step (the other elements are zero). fp16: for |x| <= 2^30 the
 // first part is at most 2^15 and leaves at most 2^18, the second is at most 2^15 and leaves at most 2^6, the
-// third is at most 2^15; what it leaves is half of its last bit, 2^-34 where that is subnormal.
+// third is at most 2^15; what it leaves is half of its last bit, 2^-34 where that is subnormal. Below 2 the first part
+// is subnormal, and the tensor core aligns a sum to the products' exponents before it adds, a subnormal's counted as
+// 2^-14: with 2^15 that costs the bits below 2^-24 (42 x 2^-24 of D at 0.01). Below 1/4 it is left out; the
+// other two hold x to 2^-22 relative, or 2^-34.
 template <typename E>
 __device__ __forceinline__ uint4 split_parts(float x) {
   if constexpr (std::is_same<E, __half>::value) {
-    const __half h0 = __float2half_rn(x * (1.0f / 32768.0f));
+    const __half h0 = __float2half_rn(fabsf(x) < 0.25f ? 0.0f : x * (1.0f / 32768.0f));
     float r = fmaf(-32768.0f, __half2float(h0), x);
     const __half h1 = __float2half_rn(r * 0.125f);
     r = fmaf(-8.0f, __half2float(h1), r) * 512.0f;

@@ -196,6 +196,20 @@ def test_attention_backward_of_large_scores(m, kind, n):
 
 
 @pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("grad", [1e-5, 1e-3, 0.05])
+def test_attention_backward_of_small_sums(m, kind, grad):
+    """Sums of dout out far below 1 beside large queries and keys: dS is a difference of them, and 0 for a single key."""
+    for H, dh in ((3, 64), (200, 16), (500, 8)):
+        lens = [1] * 20 + [2, 3, 40]
+        cu, qkv, dout = ops.attention_inputs(lens, H, dh, kind, seed=245, grad=grad)
+        qkv[:, :2 * H * dh] *= 30.0
+        scale = 0.01 / dh
+        out, lse = ops.run_forward(m, cu, qkv, H, 40, scale=scale)
+        dqkv = ops.run_backward(m, cu, qkv, H, 40, out, lse, dout, scale=scale)
+        ops.check_backward(cu, qkv, H, out, lse, dout, dqkv, scale)
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
 @pytest.mark.parametrize("terms", [1, 2, 3])
 def test_attention_backward_of_large_sums(m, kind, terms):
     """Sums of dout out up to 1e9, beside which the rest of dS is small."""
@@ -391,6 +405,47 @@ def test_attention_of_one_row_takes_any_stride(m, esm):
                                       3 * d + odd, ws.data_ptr(), size, None)
         assert rc == esm.ESM_OK, L.esm_last_error(m._ctx).decode()
         assert torch.equal(out2, out) and torch.equal(lse2, lse) and torch.equal(dqkv2, dqkv)
+
+
+def test_attention_of_the_most_heads(m):
+    for kind, dh in (("f16", 8), ("bf16", 16)):
+        H, lens = 65535, [2, 1]
+        cu, qkv, dout = ops.attention_inputs(lens, H, dh, kind, seed=404)
+        out, lse = ops.run_forward(m, cu, qkv, H, 2)
+        dqkv = ops.run_backward(m, cu, qkv, H, 2, out, lse, dout)
+        m.check_device()
+        ops.check_forward(cu, qkv, H, out, lse)
+        ops.check_backward(cu, qkv, H, out, lse, dout, dqkv)
+
+
+def test_optional_statistics(m):
+    """lse, mean and rstd may be left out; the results are the same."""
+    cu, qkv, _ = ops.attention_inputs([40, 300], 3, 40, "bf16", seed=405)
+    out, _ = ops.run_forward(m, cu, qkv, 3, 300)
+    out2 = torch.empty_like(out)
+    m.attention(qkv, cu, 300, 3, out2, stream=torch.cuda.current_stream())
+    assert torch.equal(out, out2)
+    for d in (64, 9001):
+        x, w, b = ops.ln_inputs(50, d, "f32", seed=406)
+        y, mean, rstd = ops.run_ln(m, x, w, b, "f16")
+        y2 = torch.empty_like(y)
+        m.layernorm(x, w, b, y2)
+        assert torch.equal(y, y2)
+
+
+@pytest.mark.parametrize("handle", [None, 0, 1, 2])
+def test_streams_by_their_special_handles(m, handle):
+    """The legacy default stream (null, cudaStreamLegacy) and the per-thread one."""
+    cu, qkv, dout = ops.attention_inputs([40, 300], 3, 32, "f16", seed=407)
+    out, lse = ops.run_forward(m, cu, qkv, 3, 300)
+    dqkv = ops.run_backward(m, cu, qkv, 3, 300, out, lse, dout)
+    out2, lse2, dqkv2 = torch.zeros_like(out), torch.zeros_like(lse), torch.zeros_like(dqkv)
+    ws = torch.empty(m.attention_backward_workspace(2, 340, 3), dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    m.attention(qkv, cu, 300, 3, out2, lse2, stream=handle)
+    m.attention_backward(qkv, cu, 300, 3, out2, lse2, dout, dqkv2, ws, stream=handle)
+    torch.cuda.synchronize()
+    assert torch.equal(out2, out) and torch.equal(lse2, lse) and torch.equal(dqkv2, dqkv)
 
 
 def test_distill_gradient_beside_the_logits(m):
