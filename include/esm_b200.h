@@ -254,8 +254,8 @@ int esm_matmul_tiled_noalloc(int32_t dtype, const float* d_x, const void* d_w, c
  * probabilities, and the loss of a student against a teacher's top alternatives with its gradient. (The
  * gradients of GELU and of rotary positions, and a forward that keeps what a backward pass needs, are not here.)
  *
- * All of them but esm_score, a host call like esm_forward: buffers are DEVICE memory of the context's GPU, rows are row-major, `ld` arguments
- * are row strides in elements. A call is enqueued on `stream` (a cudaStream_t of that GPU; NULL =
+ * All of them but esm_score, a host call like esm_forward: buffers are DEVICE memory of the context's GPU,
+ * rows are row-major, `ld` arguments are row strides in elements. A call is enqueued on `stream` (a cudaStream_t of that GPU; NULL =
  * the legacy default stream), allocates nothing and does not wait, so it may be captured into a CUDA
  * graph; it does not change the calling thread's current device. A null, misaligned, foreign-device
  * or host pointer, or a buffer that is written and overlaps another one, is ESM_EINVAL (column blocks of one
@@ -280,9 +280,10 @@ enum { ESM_F32 = 0, ESM_F16 = 1, ESM_BF16 = 2 };
  * rows of the buffers: rows behind the last sequence are left as they are. head_dim is a multiple of 8
  * up to 64, scale in [1e-6, 1e6]; B and n_heads are at most 65535, T at most 2^30. d_lse [H, T] or NULL (the
  * backward pass needs it). Scores, sums and outputs are accumulated in fp32, probabilities are rounded to
- * `type` for the product with V. A row with a score that is NaN or +inf has NaN in out and lse; scores of -inf
- * have probability 0 (their infinite keys still make dQ NaN in the backward pass), and a row with no other has NaN
- * in out and lse -inf; finite q k are at most 1e30 in magnitude. Offsets that do not fit (descending, beyond T or
+ * `type` for the product with V (ESM_F16: those below 2^-14 of a row's largest to 2^-25 of it). A row with a
+ * score that is NaN or +inf has NaN in out and lse; scores of -inf have probability 0 (their infinite keys still
+ * make dQ NaN in the backward pass), and a row with no other has NaN in out and lse -inf; finite q k are at most
+ * 1e30 in magnitude. Offsets that do not fit (descending, beyond T or
  * longer than max_len) are noticed on the device: that sequence, and in the backward pass perhaps others, is
  * skipped and esm_check_device returns ESM_EINVAL. */
 int esm_attention(esm_ctx* ctx, int32_t type, const void* d_qkv, int64_t ld_qkv, const int32_t* d_cu_seqlens,
@@ -353,8 +354,8 @@ int esm_score(esm_ctx* ctx, const int32_t* tokens, const int32_t* lengths, int32
  *   loss[t] = temperature^2 sum_i p_i (log p_i - log q[id_i]),  temperature in [1e-6, 100].
  * The terms are taken in fp32, so the loss has an absolute error of up to temperature^2 2^-18 beside its rounding.
  * An alternative whose id is outside [0, V) is absent, and its d_top_logits entry is ignored; a row
- * without any (or with nothing but -inf) has loss 0; a NaN shows in the loss and gradient. An id that is given twice counts with both its
- * probabilities. d_lse[t] = log sum_j exp(logits[t, j] / temperature), for the gradient. */
+ * without any (or with nothing but -inf) has loss 0; a NaN shows in the loss and gradient. An id that is given
+ * twice counts with both its probabilities. d_lse[t] = log sum_j exp(logits[t, j] / temperature), for the gradient. */
 int esm_distill_loss(esm_ctx* ctx, int32_t type, const void* d_logits, int64_t ld, int32_t T, int32_t V,
                      const int32_t* d_top_ids, const float* d_top_logits, int32_t k, float temperature, float* d_loss,
                      float* d_lse, void* stream);
